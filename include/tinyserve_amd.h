@@ -294,6 +294,52 @@ int ts_add_rms_norm(const void* x, int64_t x_stride, const float* partial, int k
                     void* x_out, int64_t xo_stride, void* h, int h_tiled, int64_t h_stride, int M,
                     int N, float eps, int dtype, void* stream);
 
+/*
+ * Rows of T x N elements quantised to 8 bits, one scale per row; row t stands for q[t] * scale[t].
+ * No counterpart in the reference's kernels. `form`:
+ *   TS_INT8_PLAIN (0):    v = x
+ *   TS_INT8_NORM (1):     v = x / sqrt(mean(x^2) + eps) * w, float32 throughout
+ *   TS_INT8_ADD_NORM (2): x = (dtype)(x + y) in place, then as TS_INT8_NORM
+ *   TS_INT8_SILU (3):     x [T, 2N] = [gate | up]; v = gate / (1 + exp(-gate)) * up, float32
+ * with a = max |v| of the row: q = rint(v * (127 / a)), scale = a / 127 (under a norm both are
+ * taken without the row's common factor, which goes into the scale). A row with a < 2^-100
+ * (before that factor) gets zeros and scale 0; a row with a NaN or an infinity, or whose sum of
+ * squares is past float32, gets zeros and scale NaN.
+ * x, y and w share `dtype`; any strides and alignment of theirs. q: 16-byte aligned, q_stride a
+ * multiple of 16 and at least N rounded up to 16; bytes of a row past N may be written. y may be
+ * x or lie beside it in the same rows; an x whose rows overlap each other's or y's is TS_EINVAL.
+ */
+#define TS_INT8_MAX_DIM (1 << 30) /* rows or columns of one 8-bit call; more is TS_EINVAL */
+#define TS_INT8_PLAIN 0
+#define TS_INT8_NORM 1
+#define TS_INT8_ADD_NORM 2
+#define TS_INT8_SILU 3
+int ts_int8_quantize_rows(void* x, const void* y, const void* w, int8_t* q, float* scale, int T,
+                          int N, int64_t x_stride, int64_t y_stride, int64_t q_stride, float eps,
+                          int form, int dtype, void* stream);
+
+/*
+ * out[t] = (dtype)(table[ids[t]] * scale[ids[t]]) for T rows of N columns of an 8-bit table of
+ * table_rows rows; ids NULL: row t itself. An id outside the table gives a row of NaN. No
+ * counterpart in the reference's kernels (its embedding is an index of the weight,
+ * src/tinyserve/model.py:181-211).
+ */
+int ts_int8_embedding(const int8_t* table, int64_t t_stride, const float* scale,
+                      int64_t table_rows, const int64_t* ids, void* out, int64_t o_stride, int T,
+                      int N, int dtype, void* stream);
+
+/*
+ * out[m, n] = (dtype)((float)(sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n]): the product of
+ * 8-bit rows x [M, K] and W [N, K] with a scale for each token and each channel. The int32 sums
+ * are exact, so out does not depend on how the work is split. K at most TS_INT8_MAX_K; any
+ * strides and alignment. K == 0 multiplies zero by the scales. No counterpart in the
+ * reference's kernels (F.linear of the decoder layer, model.py:137-179).
+ */
+#define TS_INT8_MAX_K 131071
+int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w,
+                   int64_t w_stride, const float* w_scale, void* out, int64_t o_stride, int M,
+                   int N, int K, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

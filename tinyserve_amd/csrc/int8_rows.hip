@@ -1,0 +1,407 @@
+// Rows in 8 bits on gfx950: quantisation with one scale per row (as the rows stand, after the
+// residual add and RMSNorm, after SiLU x up), and the lookup of rows of an 8-bit table.
+//
+// No kernel of the reference corresponds: its model runs in one 16- or 32-bit type
+// (src/tinyserve/model.py:137-179). These feed the 8-bit projections of int8_linear.hip.
+//
+// Quantisation of a row v:
+//   a = max |v|;  q = rint(v * (127 / a)) in -127 .. 127;  scale = a / 127
+// so that q * scale is within half a step, a / 254, of v. Two rows have no such a: one whose a
+// is below 2^-100 (127 / a could overflow) is all zeros with scale 0, and one that holds a NaN
+// or an infinity gets zeros and a NaN scale, so that whatever is computed from it is NaN, as it
+// would be in floating point.
+//
+// RMSNorm: the row is x * r * w with r = 1 / sqrt(mean x^2 + eps). r is common to the row, so it
+// cancels in q: v = x * w is quantised and r goes into the scale, (a / 127) * r. Nothing is
+// rounded between the norm and the 8 bits, and the codes do not wait for the sum of squares.
+// A row whose sum of squares leaves float32 is a NaN row. With the residual add, x = (T)(x + y)
+// is written back in place first, rounded to T as the rest of the framework holds it.
+//
+// SiLU x up: v = g / (1 + exp(-g)) * u in float32, not rounded to T in between.
+//
+// All are bound by HBM: each input is read once into registers (both maxima and sums are taken
+// there), each output written once.
+#include "common.h"
+
+namespace ts {
+
+enum Int8Form { kPlain = 0, kNorm = 1, kAddNorm = 2, kSilu = 3 };
+
+constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kTinyBits = 0x0d800000u;  // 2^-100
+
+// 16 bytes at any address: the same global_load / store_dwordx4 (gfx950 takes unaligned ones).
+typedef u32x4 u32x4_loose __attribute__((aligned(1), may_alias));
+
+template <typename T>
+__device__ __forceinline__ Pack16<T> load16_loose(const T* p) {
+  Pack16<T> r;
+  r.raw = *reinterpret_cast<const u32x4_loose*>(p);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store16_loose(T* p, const Pack16<T>& x) {
+  *reinterpret_cast<u32x4_loose*>(p) = x.raw;
+}
+
+// Elements i .. i + E - 1 of a row of N >= E elements, zeros past its end. The load itself is
+// moved back to the row's last whole vector and its elements shifted down: no branch, so the
+// loads of a row's chunks are all in flight together.
+template <typename T>
+__device__ __forceinline__ Pack16<T> load_chunk(const T* row, int i, int N) {
+  constexpr int E = Pack16<T>::N;
+  const int at = min(i, N - E);
+  Pack16<T> r = load16_loose(row + at);
+  if (N % E) {
+    const int bits = (i - at) * static_cast<int>(sizeof(T)) * 8;
+    unsigned __int128 v = static_cast<unsigned __int128>(r.raw[3]) << 96 | static_cast<unsigned __int128>(r.raw[2]) << 64 |
+                          static_cast<unsigned __int128>(r.raw[1]) << 32 | r.raw[0];
+    v = bits < 128 ? v >> (bits & 127) : 0;
+    r.raw = u32x4{static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32), static_cast<uint32_t>(v >> 64),
+                  static_cast<uint32_t>(v >> 96)};
+  } else if (i >= N) {
+    r.raw = u32x4{0, 0, 0, 0};
+  }
+  return r;
+}
+
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+
+// |v| as bits: ordered as the magnitudes are, infinities above every finite value and NaN above
+// those, so one unsigned maximum carries all three.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+template <int OFF>
+__device__ __forceinline__ uint32_t xor_lane_u(uint32_t x) {
+  return __float_as_uint(xor_lane<OFF>(__uint_as_float(x)));
+}
+
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+  x = max(x, xor_lane_u<1>(x));
+  x = max(x, xor_lane_u<2>(x));
+  x = max(x, xor_lane_u<4>(x));
+  x = max(x, xor_lane_u<8>(x));
+  x = max(x, xor_lane_u<16>(x));
+  return max(x, xor_lane_u<32>(x));
+}
+
+// A row's factor for its codes (0: all codes are zero) and its scale, from the largest
+// magnitude, and for a norm the sum of squares.
+struct RowScale {
+  float inv, scale;
+};
+
+template <int FORM>
+__device__ __forceinline__ RowScale row_scale(uint32_t top, float ss, int N, float eps) {
+  RowScale r;
+  const float a = __uint_as_float(top);
+  const bool zero = top < kTinyBits;
+  r.inv = zero ? 0.0f : 127.0f / a;
+  r.scale = zero ? 0.0f : a / 127.0f;
+  if constexpr (FORM == kNorm || FORM == kAddNorm) {
+    if (!zero) r.scale *= 1.0f / sqrtf(ss / static_cast<float>(N) + eps);
+  }
+  // top >= inf: an infinity or a NaN in the row; a scale that is not finite: a sum of squares
+  // past float32, or eps 0 under one that underflows.
+  if (top >= kInfBits || magnitude(r.scale) >= kInfBits || (FORM != kPlain && FORM != kSilu && magnitude(ss) >= kInfBits)) {
+    r.inv = 0.0f;
+    r.scale = __uint_as_float(0x7fc00000u);
+  }
+  return r;
+}
+
+// The code of v, in the low byte. A NaN row has inv 0, and 0 * inf or NaN is masked by it.
+__device__ __forceinline__ uint32_t code(float v, float inv) {
+  return static_cast<uint32_t>(static_cast<int>(rintf(inv == 0.0f ? 0.0f : v * inv))) & 0xffu;
+}
+
+struct QuantArgs {
+  const void* x;  // [T, N] (kSilu: [T, 2N], gate | up)
+  void* xo;       // kAddNorm: x again, written
+  const void* y;
+  const void* w;
+  int8_t* q;
+  float* scale;
+  int rows, N;
+  int64_t xs, ys, qs;
+  float eps;
+};
+
+// WAVES waves per row (WAVES == 1: the workgroup's waves take a row each), CPT chunks of E
+// elements per lane.
+template <typename T, int FORM, int WAVES, int CPT>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void quantize_rows_kernel(const QuantArgs a) {
+  constexpr int E = Pack16<T>::N;
+  constexpr int TPR = WAVES * kWave;
+  const int wave = threadIdx.x / kWave;
+  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWave) + wave : blockIdx.x;
+  const int t = WAVES == 1 ? threadIdx.x % kWave : threadIdx.x;
+  if (WAVES == 1 && row >= a.rows) return;
+  const int N = a.N;
+  const T* x = static_cast<const T*>(a.x) + row * a.xs;
+  const T* y = static_cast<const T*>(a.y) + row * a.ys;  // kAddNorm
+  const T* w = static_cast<const T*>(a.w);
+
+  Pack16<T> xv[CPT], sv[CPT], wv[CPT];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    const int i = (c * TPR + t) * E;
+    xv[c] = load_chunk(x, i, N);
+    if constexpr (FORM == kAddNorm) sv[c] = load_chunk(y, i, N);
+    if constexpr (FORM == kSilu) sv[c] = load_chunk(x + N, i, N);
+    if constexpr (FORM == kNorm || FORM == kAddNorm) wv[c] = load_chunk(w, i, N);
+  }
+
+  float v[CPT][E];
+  uint32_t top = 0;
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    if constexpr (FORM == kAddNorm) {
+      const int i = (c * TPR + t) * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) xv[c].v[e] = from_f32<T>(to_f32(xv[c].v[e]) + to_f32(sv[c].v[e]));
+      T* xo = static_cast<T*>(a.xo) + row * a.xs + i;
+      if (i + E <= N) {
+        store16_loose(xo, xv[c]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (i + e < N) xo[e] = xv[c].v[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float f = to_f32(xv[c].v[e]);
+      if constexpr (FORM == kSilu) f = silu(f) * to_f32(sv[c].v[e]);
+      if constexpr (FORM == kNorm || FORM == kAddNorm) {
+        ss = fmaf(f, f, ss);
+        f *= to_f32(wv[c].v[e]);
+      }
+      v[c][e] = f;
+      top = max(top, magnitude(f));
+    }
+  }
+
+  top = wave_umax(top);
+  if constexpr (FORM == kNorm || FORM == kAddNorm) ss = group_sum<kWave>(ss);
+  if constexpr (WAVES > 1) {
+    __shared__ uint32_t tops[WAVES];
+    __shared__ float sums[WAVES];
+    if (threadIdx.x % kWave == 0) {
+      tops[wave] = top;
+      sums[wave] = ss;
+    }
+    __syncthreads();
+    top = 0;
+    ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {  // in the waves' order in every thread
+      top = max(top, tops[k]);
+      ss += sums[k];
+    }
+  }
+  const RowScale r = row_scale<FORM>(top, ss, N, a.eps);
+  if (t == 0) a.scale[row] = r.scale;
+
+  int8_t* q = a.q + row * a.qs;
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    const int i = (c * TPR + t) * E;
+    if (i >= N) continue;
+    uint32_t word[E / 4];
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k)
+      word[k] = code(v[c][4 * k], r.inv) | code(v[c][4 * k + 1], r.inv) << 8 | code(v[c][4 * k + 2], r.inv) << 16 |
+                code(v[c][4 * k + 3], r.inv) << 24;
+    // Whole words: the row's padding, up to its stride, takes zeros.
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(q + i) = uint2{word[0], word[1]};
+    else *reinterpret_cast<uint32_t*>(q + i) = word[0];
+  }
+}
+
+// Any row length, one element at a time: rows shorter than one 16-byte vector, and rows longer
+// than a workgroup's registers hold, which are read twice.
+template <typename T, int FORM>
+__global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs a) {
+  const int64_t row = blockIdx.x;
+  const int N = a.N, wave = threadIdx.x / kWave;
+  const T* x = static_cast<const T*>(a.x) + row * a.xs;
+  T* xo = static_cast<T*>(a.xo) + row * a.xs;
+  const T* y = static_cast<const T*>(a.y) + row * a.ys;
+  const T* w = static_cast<const T*>(a.w);
+  // kAddNorm: the second pass reads the sums that this same thread wrote in the first.
+  auto value = [&](int i, float f) {
+    if constexpr (FORM == kSilu) return silu(f) * to_f32(x[N + i]);
+    else if constexpr (FORM == kPlain) return f;
+    else return f * to_f32(w[i]);
+  };
+  uint32_t top = 0;
+  float ss = 0.f;
+  for (int i = threadIdx.x; i < N; i += 1024) {
+    float f;
+    if constexpr (FORM == kAddNorm) {
+      const T s = from_f32<T>(to_f32(xo[i]) + to_f32(y[i]));
+      xo[i] = s;
+      f = to_f32(s);
+    } else {
+      f = to_f32(x[i]);
+    }
+    if constexpr (FORM == kNorm || FORM == kAddNorm) ss = fmaf(f, f, ss);
+    top = max(top, magnitude(value(i, f)));
+  }
+  top = wave_umax(top);
+  ss = group_sum<kWave>(ss);
+  __shared__ uint32_t tops[16];
+  __shared__ float sums[16];
+  if (threadIdx.x % kWave == 0) {
+    tops[wave] = top;
+    sums[wave] = ss;
+  }
+  __syncthreads();
+  top = 0;
+  ss = 0.f;
+  for (int k = 0; k < 16; ++k) {
+    top = max(top, tops[k]);
+    ss += sums[k];
+  }
+  const RowScale r = row_scale<FORM>(top, ss, N, a.eps);
+  if (threadIdx.x == 0) a.scale[row] = r.scale;
+  int8_t* q = a.q + row * a.qs;
+  for (int i = threadIdx.x; i < N; i += 1024) {
+    float f;
+    if constexpr (FORM == kAddNorm) f = to_f32(xo[i]);
+    else f = to_f32(x[i]);
+    q[i] = static_cast<int8_t>(code(value(i, f), r.inv));
+  }
+}
+
+template <typename T, int FORM>
+static int launch_quantize(const QuantArgs& a, hipStream_t st) {
+  constexpr int E = Pack16<T>::N;
+  const int chunks = (a.N + E - 1) / E;
+  const bool few = a.rows < 2 * compute_units();
+#define TS_QUANT(W, C)                                                                                     \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, W, C>), dim3((W) == 1 ? (a.rows + 3) / 4 : a.rows),    \
+                     dim3((W) == 1 ? 256 : (W) * kWave), 0, st, a)
+  if (a.N < E || chunks > 4096) hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(1024), 0, st, a);
+  else if (chunks <= 64) TS_QUANT(1, 1);
+  else if (few && chunks <= 256) TS_QUANT(4, 1);
+  else if (few && chunks <= 512) TS_QUANT(4, 2);
+  else if (chunks <= 128) TS_QUANT(1, 2);
+  else if (chunks <= 256) TS_QUANT(1, 4);
+  else if (chunks <= 512) TS_QUANT(4, 2);
+  else if (chunks <= 1024) TS_QUANT(4, 4);
+  else if (chunks <= 2048) TS_QUANT(16, 2);
+  else TS_QUANT(16, 4);
+#undef TS_QUANT
+  return launch_status();
+}
+
+template <typename T>
+static int launch_form(const QuantArgs& a, int form, hipStream_t st) {
+  switch (form) {
+    case kPlain: return launch_quantize<T, kPlain>(a, st);
+    case kNorm: return launch_quantize<T, kNorm>(a, st);
+    case kAddNorm: return launch_quantize<T, kAddNorm>(a, st);
+    default: return launch_quantize<T, kSilu>(a, st);
+  }
+}
+
+// ---- rows of an 8-bit table -----------------------------------------------------------------
+// out[t] = (T)(q[ids[t]] * scale[ids[t]]): one thread per 16 codes. Bound by HBM (and, for few
+// ids, by the chain id -> row). An id outside the table gives a row of NaN.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_embedding_kernel(const int8_t* __restrict__ q, int64_t qs,
+                                                             const float* __restrict__ scale, int64_t table,
+                                                             const int64_t* __restrict__ ids, T* __restrict__ out,
+                                                             int64_t os, int rows, int N, int per_row) {
+  const int64_t total = static_cast<int64_t>(rows) * per_row;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t t = u / per_row;
+    const int i = static_cast<int>(u - t * per_row) * 16;
+    const int64_t id = ids ? ids[t] : t;
+    const bool in = id >= 0 && id < table;
+    const float s = in ? scale[id] : __uint_as_float(0x7fc00000u);
+    const int8_t* p = q + (in ? id : 0) * qs + i;
+    T* o = out + t * os + i;
+    if (i + 16 <= N) {
+      union {
+        u32x4 raw;
+        int8_t b[16];
+      } c;
+      c.raw = load16_loose(p).raw;
+      constexpr int E = Pack16<T>::N;
+#pragma unroll
+      for (int k = 0; k < 16 / E; ++k) {
+        Pack16<T> y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y.v[e] = from_f32<T>(static_cast<float>(c.b[k * E + e]) * s);
+        store16_loose(o + k * E, y);
+      }
+    } else {
+      for (int e = 0; e < N - i; ++e) o[e] = from_f32<T>(static_cast<float>(p[e]) * s);
+    }
+  }
+}
+
+template <typename T>
+static int launch_embedding(const int8_t* q, int64_t qs, const float* scale, int64_t table, const int64_t* ids, void* out,
+                            int64_t os, int rows, int N, hipStream_t st) {
+  const int per_row = (N + 15) / 16;
+  const int64_t blocks = (static_cast<int64_t>(rows) * per_row + 255) / 256;
+  hipLaunchKernelGGL(int8_embedding_kernel<T>, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256),
+                     0, st, q, qs, scale, table, ids, static_cast<T*>(out), os, rows, N, per_row);
+  return launch_status();
+}
+
+}  // namespace ts
+
+using namespace ts;
+
+extern "C" int ts_int8_quantize_rows(void* x, const void* y, const void* w, int8_t* q, float* scale, int T, int N,
+                                     int64_t x_stride, int64_t y_stride, int64_t q_stride, float eps, int form, int dtype,
+                                     void* stream) {
+  if (T < 0 || T > TS_INT8_MAX_DIM || N <= 0 || N > TS_INT8_MAX_DIM || form < kPlain || form > kSilu) return TS_EINVAL;
+  const int64_t padded = (static_cast<int64_t>(N) + 15) / 16 * 16;
+  if (q_stride < padded || q_stride % 16 || reinterpret_cast<uintptr_t>(q) % 16) return TS_EINVAL;
+  if (dtype < TS_F32 || dtype > TS_BF16) return TS_EUNSUPPORTED;
+  if (T == 0) return 0;
+  if (!x || !q || !scale || x_stride < 0) return TS_EINVAL;
+  if ((form == kNorm || form == kAddNorm) && !w) return TS_EINVAL;
+  if (form == kAddNorm) {
+    // x is written: its rows may not overlap each other, nor y's, unless y is x itself or lies
+    // beside it in the same rows.
+    if (!y || y_stride < 0 || (T > 1 && x_stride < N)) return TS_EINVAL;
+    const int64_t es = elem_size(dtype);
+    const int64_t x0 = reinterpret_cast<int64_t>(x), y0 = reinterpret_cast<int64_t>(y);
+    const int64_t x1 = x0 + ((T - 1) * x_stride + N) * es, y1 = y0 + ((T - 1) * y_stride + N) * es;
+    if (x0 < y1 && y0 < x1 && !(x0 == y0 && (x_stride == y_stride || T == 1))) {
+      const int64_t pitch = x_stride * es, d = T > 1 && x_stride == y_stride ? ((y0 - x0) % pitch + pitch) % pitch : 0;
+      if (T == 1 || x_stride != y_stride || d < N * es || d > pitch - N * es) return TS_EINVAL;
+    }
+  }
+  const QuantArgs a{x, x, y, w, q, scale, T, N, x_stride, y_stride, q_stride, eps};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TS_F32: return launch_form<float>(a, form, st);
+    case TS_F16: return launch_form<f16>(a, form, st);
+    default: return launch_form<bf16>(a, form, st);
+  }
+}
+
+extern "C" int ts_int8_embedding(const int8_t* table, int64_t t_stride, const float* scale, int64_t table_rows,
+                                 const int64_t* ids, void* out, int64_t o_stride, int T, int N, int dtype, void* stream) {
+  if (T < 0 || T > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM || t_stride < 0 || table_rows < 0 || (T > 1 && o_stride < N)) return TS_EINVAL;
+  if (dtype < TS_F32 || dtype > TS_BF16) return TS_EUNSUPPORTED;
+  if (T == 0 || N == 0) return 0;
+  // The rows of an empty table do not exist: there is nothing to read for any id.
+  if (!table || !scale || !out || table_rows == 0 || (!ids && T > table_rows)) return TS_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TS_F32: return launch_embedding<float>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
+    case TS_F16: return launch_embedding<f16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
+    default: return launch_embedding<bf16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
+  }
+}

@@ -1,0 +1,208 @@
+"""The 8-bit integer path of a step's projections on MI355X (``csrc/int8_rows.hip``,
+``csrc/int8_linear.hip``): activations quantised per token, weights per output channel, their
+products on the int8 matrix cores.
+
+A decoder layer's projections (src/tinyserve/model.py:137-179) with 8-bit weights:
+
+    h    = rms_norm(x)                  rms_norm_rows_int8(x, w, eps)
+    qkv  = F.linear(h, W_qkv)           int8_linear(h, W_qkv, dtype)
+    x    = x + F.linear(attn, W_o)      y = int8_linear(quantize_rows(attn), W_o, dtype)
+    h    = rms_norm(x)                  add_rms_norm_rows_int8(x, y, w, eps)   (x updated)
+    act  = silu(gate) * up              silu_mul_int8(int8_linear(h, W_gate_up, dtype))
+    x    = x + F.linear(act, W_down)    int8_linear(act, W_down, dtype), added by the next norm
+
+``Int8Rows`` holds such a matrix: codes ``q`` (int8 ``[M, K]``) and one float32 ``scale`` per
+row; it stands for ``q * scale[:, None]``. Weights ``[N, K]`` are quantised once by
+``quantize_rows(w)``. The reference keeps every weight in one float type, so no function of it
+corresponds. These are for inference: no gradient flows through them.
+
+Every launch goes on torch's current stream of the inputs' device, never synchronises, and
+allocates only its results, by torch's caching allocator, so a HIP graph can capture them.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from tinyserve_amd import _lib
+
+PLAIN, NORM, ADD_NORM, SILU = 0, 1, 2, 3
+MAX_K = 131071  # products of longer rows could pass an int32
+MAX_DIM = 1 << 30  # rows or columns of one call
+
+
+class Int8Rows(NamedTuple):
+    """An 8-bit matrix with one scale per row: ``q`` int8 ``[M, K]``, unit column stride,
+    ``scale`` float32 ``[M]``. A row with a NaN scale stands for NaN."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def _call(dev: int, name: str, *args: object) -> None:
+    """Launch on ``dev``'s current stream, whichever device is current."""
+    if torch._C._cuda_getDevice() == dev:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _check_matrix(x: torch.Tensor, what: str) -> None:
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"{what} must be a row-contiguous [T, N] tensor, got {tuple(x.shape)}")
+    if x.dtype not in _lib.DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype}: float32, float16 or bfloat16")
+    _check_dims(x, what)
+
+
+def _check_dims(x: torch.Tensor, what: str) -> None:
+    if x.shape[0] > MAX_DIM or x.shape[1] > MAX_DIM:
+        raise ValueError(f"{what}: at most {MAX_DIM} rows and columns, got {tuple(x.shape)}")
+
+
+def _check_weight(weight: torch.Tensor, x: torch.Tensor) -> None:
+    if weight.shape != (x.shape[1],) or weight.dtype != x.dtype or not weight.is_contiguous():
+        raise ValueError(f"the weight must be a contiguous {x.dtype} vector of {x.shape[1]}, "
+                         f"got {weight.dtype} {tuple(weight.shape)}")  # fmt: skip
+
+
+def _check_rows(r: Int8Rows, what: str) -> None:
+    q, scale = r
+    if q.dtype != torch.int8 or q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1):
+        raise ValueError(f"{what}: codes must be row-contiguous int8 [M, K], got {q.dtype} {tuple(q.shape)}")
+    _check_dims(q, what)
+    if scale.dtype != torch.float32 or scale.shape != (q.shape[0],) or not scale.is_contiguous():
+        raise ValueError(f"{what}: scales must be contiguous float32 [{q.shape[0]}], got {scale.dtype} {tuple(scale.shape)}")
+
+
+def _quantize(form: int, x: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor | None, eps: float,
+              n: int) -> Int8Rows:  # fmt: skip
+    """One launch of ``ts_int8_quantize_rows``. Codes' rows start at multiples of 16 bytes."""
+    t = x.shape[0]
+    dev = _lib.require_device(x, *(z for z in (y, weight) if z is not None))
+    q = torch.empty((t, (n + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+    scale = torch.empty(t, dtype=torch.float32, device=x.device)
+    if t and n:
+        _call(dev, "ts_int8_quantize_rows", x.data_ptr(), None if y is None else y.data_ptr(),
+              None if weight is None else weight.data_ptr(), q.data_ptr(), scale.data_ptr(), t, n, x.stride(0),
+              0 if y is None else y.stride(0), q.stride(0), eps, form, _lib.DTYPES[x.dtype])  # fmt: skip
+    elif t:
+        scale.zero_()  # rows of no columns
+    return Int8Rows(q if q.shape[1] == n else q[:, :n], scale)
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """Rows of ``x [T, N]`` in 8 bits: ``a = max|x[t]|``, ``q = rint(x * (127 / a))``,
+    ``scale = a / 127``. A row of zeros (or below 2^-100) gets scale 0, one that holds a NaN or
+    an infinity scale NaN; both get zero codes."""
+    _check_matrix(x, "x")
+    return _quantize(PLAIN, x, None, None, 0.0, x.shape[1])
+
+
+def rms_norm_rows_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> Int8Rows:
+    """``quantize_rows`` of RMSNorm of each row of ``x``, in one launch. The norm is not rounded
+    to x's dtype before it is quantised (``rms_norm_rows`` rounds twice). ``eps`` is positive."""
+    _check_matrix(x, "x")
+    _check_weight(weight, x)
+    return _quantize(NORM, x, None, weight, _eps(eps), x.shape[1])
+
+
+def add_rms_norm_rows_int8(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: float) -> Int8Rows:
+    """``x.add_(y)``, rounded to its dtype, then ``rms_norm_rows_int8(x, weight, eps)``, in one
+    launch. ``x`` is updated in place; its rows must not overlap each other's, nor ``y``'s unless
+    ``y`` is ``x``."""
+    _check_matrix(x, "x")
+    _check_weight(weight, x)
+    if y.shape != x.shape or y.dtype != x.dtype or (y.stride(1) != 1 and y.shape[1] > 1):
+        raise ValueError(f"y must be row-contiguous {tuple(x.shape)} {x.dtype}, got {tuple(y.shape)} {y.dtype}")
+    return _quantize(ADD_NORM, x, y, weight, _eps(eps), x.shape[1])
+
+
+def _eps(eps: float) -> float:
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps}")
+    return float(eps)
+
+
+def silu_mul_int8(gate_up: torch.Tensor) -> Int8Rows:
+    """``quantize_rows(F.silu(gate) * up)`` of ``[gate | up]`` rows ``[T, 2N]``, in one launch,
+    in float32 up to the 8 bits (``silu_mul`` rounds each factor to the dtype)."""
+    _check_matrix(gate_up, "gate_up")
+    if gate_up.shape[1] % 2:
+        raise ValueError(f"need [gate | up] rows of an even width, got {tuple(gate_up.shape)}")
+    return _quantize(SILU, gate_up, None, None, 0.0, gate_up.shape[1] // 2)
+
+
+def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``F.linear`` of 8-bit rows: ``(q_x . q_w^T) * scale_x[:, None] * scale_w``, ``[M, N]`` in
+    ``dtype``. The integer sums are exact and rounded to float32 once.
+
+    Args:
+        x: ``[M, K]`` tokens. w: ``[N, K]`` weights, a scale per output channel. K up to 131071;
+            rows that start at multiples of 16 bytes, as the functions here make them, are
+            read fastest.
+        out: ``[M, N]`` in ``dtype``, unit column stride (default: a new tensor).
+    """
+    xq, xs = x
+    wq, ws = w
+    _check_rows(x, "x")
+    _check_rows(w, "w")
+    m, k = xq.shape
+    n = wq.shape[0]
+    if wq.shape[1] != k:
+        raise ValueError(f"x has {k} columns but w is {tuple(wq.shape)}")
+    if k > MAX_K:
+        raise ValueError(f"K is at most {MAX_K} (the sums are int32), got {k}")
+    code = _lib.DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
+    dev = _lib.require_device(xq, xs, wq, ws)
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=xq.device)
+    else:
+        if out.shape != (m, n) or out.dtype != dtype or (out.stride(1) != 1 and n > 1) or (m > 1 and out.stride(0) < n):
+            raise ValueError(f"out must be {dtype} [{m}, {n}] with unit column stride, got {out.dtype} {tuple(out.shape)}")
+        if _lib.require_device(out) != dev:
+            raise ValueError("out is on another device")
+    if m and n:
+        _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+              ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, code)  # fmt: skip
+    return out
+
+
+def int8_embedding(table: Int8Rows, ids: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Rows ``ids`` of an 8-bit table as ``dtype``: ``table.q[ids] * table.scale[ids][:, None]``,
+    ``[T, N]``, rounded once. ids: int64 ``[T]`` (int32 is accepted and widened); an id outside
+    the table gives a row of NaN."""
+    if ids.dim() != 1 or ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"ids must be a [T] int64 or int32 tensor, got {ids.dtype} {tuple(ids.shape)}")
+    return _rows_of(table, ids, dtype)
+
+
+def dequantize_rows(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
+    """The values that ``rows`` stands for, ``q * scale[:, None]``, in ``dtype``, rounded once."""
+    return _rows_of(rows, None, dtype)
+
+
+def _rows_of(table: Int8Rows, ids: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
+    q, scale = table
+    _check_rows(table, "table")
+    code = _lib.DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
+    v, n = q.shape
+    t = v if ids is None else ids.shape[0]
+    if t and not v:
+        raise ValueError("the table has no rows")
+    if t > MAX_DIM:
+        raise ValueError(f"at most {MAX_DIM} ids, got {t}")
+    dev = _lib.require_device(q, scale) if ids is None else _lib.require_device(q, scale, ids)
+    out = torch.empty((t, n), dtype=dtype, device=q.device)
+    if t and n:
+        at = None if ids is None else ids.to(torch.int64).contiguous()
+        _call(dev, "ts_int8_embedding", q.data_ptr(), q.stride(0), scale.data_ptr(), v, _lib.ptr(at), out.data_ptr(),
+              out.stride(0), t, n, code)  # fmt: skip
+    return out
