@@ -51,6 +51,21 @@ __device__ __forceinline__ void store16(T* p, const Pack16<T>& x) {
   *reinterpret_cast<u32x4*>(p) = x.raw;
 }
 
+// 16 bytes at any address: the same global_load / store_dwordx4 (gfx950 takes unaligned ones).
+typedef u32x4 u32x4_loose __attribute__((aligned(1), may_alias));
+
+template <typename T>
+__device__ __forceinline__ Pack16<T> load16_loose(const T* p) {
+  Pack16<T> r;
+  r.raw = *reinterpret_cast<const u32x4_loose*>(p);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store16_loose(T* p, const Pack16<T>& x) {
+  *reinterpret_cast<u32x4_loose*>(p) = x.raw;
+}
+
 // x from the lane whose id is (this lane's id) XOR OFF. OFF < 32 stays inside a
 // 32-lane half and uses ds_swizzle's xor mode (no address computation); OFF == 32
 // crosses the halves through ds_bpermute.
@@ -63,6 +78,37 @@ __device__ __forceinline__ float xor_lane(float x) {
     constexpr int pattern = (OFF << 10) | 0x1f;  // and_mask 31, or_mask 0, xor_mask OFF
     return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), pattern));
   }
+}
+
+#define TS_LDS __attribute__((address_space(3)))
+
+// One direct-to-LDS load of 16 bytes per lane with a scalar base address and a 32-bit
+// per-lane byte offset (global_load_lds_dwordx4 voffset, saddr): lane l's bytes land at
+// dst + 16 l. Inline asm, since the compiler's wait-count pass would guard every later LDS
+// read with a wait for all such loads in flight; the kernel orders them itself with counted
+// waits before its barriers.
+// M0 is bound through the asm operand, so the compiler sets it (one instruction) and
+// knows it is taken.
+__device__ __forceinline__ void lds_load16_s(const void* base, uint32_t voff, TS_LDS void* dst) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst));
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "{m0}"(lds) : "memory");
+#endif
+}
+
+// Wait until at most N of this wave's vector-memory operations are in flight and all its
+// LDS operations are done, then meet the other waves at s_barrier. __syncthreads() would
+// also fence workgroup memory, which waits for every load in flight (vmcnt(0)) and so
+// drains the ring; the tiles' visibility needs only each wave's own counted wait. The
+// signal fences (no instructions) keep the compiler from moving memory accesses across.
+template <int N>
+__device__ __forceinline__ void ring_barrier() {
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  // vmcnt N (bits 3:0 and 15:14), expcnt 7 (no wait), lgkmcnt 0
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 // Sum / max over groups of N consecutive lanes (N a power of 2 <= 64); every lane of a

@@ -14,7 +14,7 @@
 namespace ts {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_loose __attribute__((aligned(1), may_alias));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 struct LinearArgs {
   const int8_t* x;
@@ -165,11 +165,225 @@ static int launch_rows8(const LinearArgs& a, hipStream_t st) {
   return launch_status();
 }
 
+// ---- many rows: tiles through LDS -------------------------------------------------------------
+// Each of the workgroup's GM x GN waves takes 32 MW rows of x and 32 NW rows of W: MW * NW
+// accumulators of v_mfma_i32_32x32x32_i8, W the A operand and x the B operand.
+//
+// Both operands go through a ring of kStages LDS tiles of 64 columns, filled by direct-to-LDS
+// loads (four lanes per row of 64 bytes) while older tiles are multiplied. Row r's 16-byte unit c
+// sits in slot c ^ swizzle(r), which spreads any 8 or 16 rows' units c over all banks; the lanes
+// of a load fetch the units that their slots hold. A step's operands are read from LDS while the
+// step before is multiplied; the barrier that hands over the next tile stands between a tile's
+// two steps, so the last product of one tile covers the first reads of the next.
+//
+// kAligned false: rows that do not start at multiples of 16 bytes go through registers instead
+// (unaligned vector loads), one tile ahead.
+//
+// The last K % 64 columns come first, alone, with zeros past the end of the rows.
+__device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+
+template <typename T, int MW, int NW, int GM, int GN, int kStages, bool kAligned>
+__global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
+  constexpr int kWaves = GM * GN, kThreads = kWaves * kWave;
+  constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
+  constexpr int kStage = (BM + BN) * 64;      // bytes: BN rows of W, then BM rows of x
+  constexpr int LPW = (BM + BN) / 16 / kWaves;  // loads per wave and tile, 16 rows each
+  constexpr int kRow = 32 * NW * sizeof(T) + 16;  // bytes of a row of the output staging
+  constexpr int kLds = kStages * kStage > kWaves * 32 * kRow ? kStages * kStage : kWaves * 32 * kRow;
+  static_assert((BM + BN) % (16 * kWaves) == 0 && kLds <= 160 * 1024, "tile shape");
+  __shared__ __attribute__((aligned(16))) int8_t lds[kLds];
+
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wm = wave / GN, wn = wave % GN;
+
+  // Workgroups go round-robin over the 8 XCDs: each XCD takes a contiguous run of tiles, in
+  // bands of 4 tiles of x, so that the tiles running on it share rows of x and W in its L2.
+  int tm, tn;
+  {
+    const int total = tiles_m * tiles_n, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
+    const int t = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    const int band = t / (4 * tiles_n), first = band * 4, high = min(4, tiles_m - first);
+    const int in = t - band * 4 * tiles_n;
+    tm = first + in % high;
+    tn = in / high;
+  }
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int8_t* wg = a.w + static_cast<int64_t>(n0) * a.ws;
+  const int8_t* xg = a.x + static_cast<int64_t>(m0) * a.xs;
+
+  // Load j of this wave fills LDS rows 16 (wave * LPW + j) .. + 15, four lanes each; rows past the
+  // ends repeat the last one (their sums are not stored).
+  auto load_row = [&](int j) { return 16 * (wave * LPW + j) + lane / 4; };
+  const int load_unit = (lane % 4) ^ swizzle(lane / 4);
+  uint32_t off[LPW];
+#pragma unroll
+  for (int j = 0; j < LPW; ++j) {
+    const int r = load_row(j);
+    const int64_t row = r < BN ? min(r, a.N - 1 - n0) * a.ws : min(r - BN, a.M - 1 - m0) * a.xs;
+    off[j] = static_cast<uint32_t>(row) + load_unit * 16;
+  }
+  // LDS bytes of unit 2 s + lane / 32 of row lane % 32 of a 32-row operand tile.
+  int unit[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) unit[s] = (lane % 32) * 64 + (((2 * s + lane / 32) ^ swizzle(lane % 32)) * 16);
+
+  i32x16 acc[NW][MW];
+#pragma unroll
+  for (int t = 0; t < NW; ++t)
+#pragma unroll
+    for (int u = 0; u < MW; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][u][i] = 0;
+
+  i32x4 wf[2][NW], xf[2][MW];  // operands of the two steps of a tile
+  auto read_w = [&](int s, int t, const int8_t* tile) {
+    wf[s][t] = *reinterpret_cast<const i32x4*>(tile + (wn * NW + t) * 2048 + unit[s]);
+  };
+  auto read_x = [&](int s, int u, const int8_t* tile) {
+    xf[s][u] = *reinterpret_cast<const i32x4*>(tile + BN * 64 + (wm * MW + u) * 2048 + unit[s]);
+  };
+  auto read_all = [&](int s, const int8_t* tile) {
+#pragma unroll
+    for (int t = 0; t < NW; ++t) read_w(s, t, tile);
+#pragma unroll
+    for (int u = 0; u < MW; ++u) read_x(s, u, tile);
+  };
+  auto multiply = [&](int s, int p) {  // product p of step s
+    acc[p / MW][p % MW] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s][p / MW], xf[s][p % MW], acc[p / MW][p % MW], 0, 0, 0);
+  };
+  auto multiply_all = [&](int s) {
+#pragma unroll
+    for (int p = 0; p < NW * MW; ++p) multiply(s, p);
+  };
+
+  const int tiles = a.K / 64;
+  if (a.K % 64) {
+#pragma unroll
+    for (int j = 0; j < LPW; ++j) {
+      const int r = load_row(j);
+      const int8_t* row = r < BN ? wg + min(r, a.N - 1 - n0) * a.ws : xg + min(r - BN, a.M - 1 - m0) * a.xs;
+      *reinterpret_cast<i32x4*>(lds + r * 64 + (lane % 4) * 16) = load_codes_tail(row, tiles * 64 + load_unit * 16, a.K);
+    }
+    __syncthreads();
+    read_all(0, lds);
+    read_all(1, lds);
+    multiply_all(0);
+    multiply_all(1);
+    __syncthreads();
+  }
+
+  if constexpr (kAligned) {
+    auto load = [&](int j, int kt, int8_t* tile) {
+      const int row0 = 16 * (wave * LPW + j);
+      const int8_t* base = (row0 < BN ? wg : xg) + static_cast<int64_t>(kt) * 64;
+      lds_load16_s(base, off[j], (TS_LDS void*)(tile + row0 * 64));
+    };
+    for (int kt = 0; kt < min(kStages, tiles); ++kt)
+#pragma unroll
+      for (int j = 0; j < LPW; ++j) load(j, kt, lds + kt * kStage);
+    if (tiles >= kStages) ring_barrier<(kStages - 1) * LPW>();
+    else ring_barrier<0>();
+    if (tiles > 0) read_all(0, lds);
+    int at = 0;  // LDS offset of tile kt
+    for (int kt = 0; kt < tiles; ++kt) {
+      int8_t* tile = lds + at;
+      at = at + kStage == kStages * kStage ? 0 : at + kStage;
+      int8_t* next = lds + at;
+      read_all(1, tile);
+      multiply_all(0);
+      // Every read of this tile is done and the next one has landed, in every wave.
+      if (kt + kStages - 1 < tiles) ring_barrier<(kStages - 2) * LPW>();
+      else ring_barrier<0>();
+      if (kt + kStages < tiles) {
+#pragma unroll
+        for (int j = 0; j < LPW; ++j) load(j, kt + kStages, tile);
+      }
+      if (kt + 1 < tiles) read_all(0, next);
+      multiply_all(1);
+    }
+  } else if (tiles > 0) {
+    i32x4 held[LPW];
+    auto fetch = [&](int kt) {
+#pragma unroll
+      for (int j = 0; j < LPW; ++j)
+        held[j] = load_codes((16 * (wave * LPW + j) < BN ? wg : xg) + static_cast<int64_t>(kt) * 64 + off[j]);
+    };
+    fetch(0);
+    for (int kt = 0; kt < tiles; ++kt) {
+      int8_t* tile = lds + (kt & 1) * kStage;
+#pragma unroll
+      for (int j = 0; j < LPW; ++j) *reinterpret_cast<i32x4*>(tile + load_row(j) * 64 + (lane % 4) * 16) = held[j];
+      if (kt + 1 < tiles) fetch(kt + 1);
+      __syncthreads();  // two tiles: the one before this is read by no wave that has passed it
+      read_all(0, tile);
+      read_all(1, tile);
+      multiply_all(0);
+      multiply_all(1);
+    }
+  }
+  __syncthreads();  // the ring's last reads, before the outputs take its place
+
+  // Lane l holds column l % 32 (a row of x) and rows 8 j + 4 (l / 32) .. + 3 (of W) of each result.
+  // 32 rows of outputs at a time go through the wave's own part of LDS and out in whole vectors.
+  int8_t* mine = lds + wave * 32 * kRow;
+  constexpr int E = Pack16<T>::N, VPR = 32 * NW / E;  // vectors per row
+#pragma unroll
+  for (int u = 0; u < MW; ++u) {
+    const int mrow = m0 + (wm * MW + u) * 32;
+    const float s = a.xscale[min(mrow + lane % 32, a.M - 1)];
+#pragma unroll
+    for (int t = 0; t < NW; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = t * 32 + j * 8 + lane / 32 * 4;
+        const int n = n0 + wn * 32 * NW + c;
+        typename Loose<T, 4>::Vec y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[i] = from_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * a.wscale[min(n + i, a.N - 1)]);
+        *reinterpret_cast<typename Loose<T, 4>::Vec*>(mine + (lane % 32) * kRow + c * sizeof(T)) = y;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int v = 0; v < 32 * VPR / kWave; ++v) {
+      const int r = (v * kWave + lane) / VPR, c = (v * kWave + lane) % VPR * E;
+      const int m = mrow + r, n = n0 + wn * 32 * NW + c;
+      const Pack16<T> y = load16(reinterpret_cast<const T*>(mine + r * kRow) + c);
+      if (m >= a.M) continue;
+      T* o = static_cast<T*>(a.out) + m * a.os + n;
+      if (n + E <= a.N) {
+        store16_loose(o, y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (n + e < a.N) o[e] = y.v[e];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <typename T, int MW, int NW, int GM, int GN, int kStages, bool kAligned>
+static int launch_tiles(const LinearArgs& a, hipStream_t st) {
+  constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
+  const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+  if (tm * tn > INT32_MAX) return TS_EUNSUPPORTED;
+  hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kStages, kAligned>), dim3(static_cast<unsigned>(tm * tn)),
+                     dim3(GM * GN * kWave), 0, st, a, static_cast<int>(tm), static_cast<int>(tn));
+  return launch_status();
+}
+
 template <typename T>
 static int launch_linear(const LinearArgs& a, hipStream_t st) {
   if (a.M <= 16) return launch_rows8<T, 8, 1, 1>(a, st);
   if (a.M <= 32) return launch_rows8<T, 8, 1, 2>(a, st);
-  return launch_rows8<T, 8, 1, 4>(a, st);
+  // Tiles address their rows by 32-bit offsets: 255 rows of at most 2^23 bytes.
+  if (a.M <= 128 || a.xs > 1 << 23 || a.ws > 1 << 23) return launch_rows8<T, 8, 1, 4>(a, st);
+  const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.xs | a.ws) & 15) == 0;
+  if (!aligned) return launch_tiles<T, 2, 2, 2, 2, 2, false>(a, st);
+  if (a.M >= 1024 && a.N >= 1024) return launch_tiles<T, 4, 4, 2, 2, 4, true>(a, st);
+  return launch_tiles<T, 2, 2, 2, 2, 4, true>(a, st);
 }
 
 }  // namespace ts

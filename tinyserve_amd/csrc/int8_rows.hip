@@ -30,21 +30,6 @@ enum Int8Form { kPlain = 0, kNorm = 1, kAddNorm = 2, kSilu = 3 };
 constexpr uint32_t kInfBits = 0x7f800000u;
 constexpr uint32_t kTinyBits = 0x0d800000u;  // 2^-100
 
-// 16 bytes at any address: the same global_load / store_dwordx4 (gfx950 takes unaligned ones).
-typedef u32x4 u32x4_loose __attribute__((aligned(1), may_alias));
-
-template <typename T>
-__device__ __forceinline__ Pack16<T> load16_loose(const T* p) {
-  Pack16<T> r;
-  r.raw = *reinterpret_cast<const u32x4_loose*>(p);
-  return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void store16_loose(T* p, const Pack16<T>& x) {
-  *reinterpret_cast<u32x4_loose*>(p) = x.raw;
-}
-
 // Elements i .. i + E - 1 of a row of N >= E elements, zeros past its end. The load itself is
 // moved back to the row's last whole vector and its elements shifted down: no branch, so the
 // loads of a row's chunks are all in flight together.

@@ -75,7 +75,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-#define TS_LDS __attribute__((address_space(3)))
 #define TS_CONST __attribute__((address_space(4)))
 
 template <typename T>
@@ -297,33 +296,6 @@ __device__ __forceinline__ void lds_load16(const void* src, TS_LDS void* dst) {
       : "s"(lds), "v"(src)
       : "memory");
 #endif
-}
-
-// The same load with a scalar base address and a 32-bit per-lane byte offset
-// (global_load_lds_dwordx4 voffset, saddr): the address arithmetic of a gather whose
-// lanes share one cache block stays on the scalar unit.
-// M0 is bound through the asm operand, so the compiler sets it (one instruction) and
-// knows it is taken.
-__device__ __forceinline__ void lds_load16_s(const void* base, uint32_t voff, TS_LDS void* dst) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst));
-  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "{m0}"(lds) : "memory");
-#endif
-}
-
-// Wait until at most N of this wave's vector-memory operations are in flight and all its
-// LDS operations are done, then meet the other waves at s_barrier. __syncthreads() would
-// also fence workgroup memory, which waits for every load in flight (vmcnt(0)) and so
-// drains the ring; the tiles' visibility needs only each wave's own counted wait. The
-// signal fences (no instructions) keep the compiler from moving memory accesses across.
-template <int N>
-__device__ __forceinline__ void ring_barrier() {
-  static_assert(N >= 0 && N < 64, "vmcnt field");
-  // vmcnt N (bits 3:0 and 15:14), expcnt 7 (no wait), lgkmcnt 0
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_barrier();
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 template <typename T, int D, int HG, int QB, int kWaves, int kStages, int kBN, int kOcc,
