@@ -183,14 +183,25 @@ def test_c_abi_refuses_before_any_launch() -> None:
                 {"y": 0x1000 - 14, "t": 1}, {"xs": 16, "ys": 16, "y": 0x1000 + 2 * 16 + 14}):  # fmt: skip
         assert quant(form=2, **bad) == -1, bad
 
-    def linear(m=2, n=3, k=4, xs=4, ws=4, os=3, dtype=1, x=0x1000, w=0x2000, out=0x3000, a=0x4000, b=0x5000):  # noqa: ANN001, ANN202
-        return lib.ts_int8_linear(x, xs, a, w, ws, b, out, os, m, n, k, dtype, None)
+    def linear(m=2, n=3, k=4, xs=4, ws=4, os=3, padded=0, dtype=1, x=0x1000, w=0x2000, out=0x3000, a=0x4000, b=0x5000):  # noqa: ANN001, ANN202
+        return lib.ts_int8_linear(x, xs, a, w, ws, b, out, os, m, n, k, padded, dtype, None)
 
     assert linear(m=0) == 0 and linear(n=0) == 0
     for bad in ({"m": -1}, {"m": big}, {"n": -1}, {"n": big}, {"k": -1}, {"k": 131072}, {"xs": -1}, {"ws": -1}, {"os": 2},
                 {"x": None}, {"w": None}, {"out": None}, {"a": None}, {"b": None}):  # fmt: skip
         assert linear(**bad) == -1, bad
     assert linear(dtype=7) == -2
+    tiled = {"m": 200, "k": 20, "xs": 32, "ws": 32}  # many rows: aligned and readable to 32 columns, or not taken
+    for bad in ({"padded": 0}, {"padded": 1, "xs": 20}, {"padded": 1, "ws": 24}, {"padded": 1, "x": 0x1008},
+                {"padded": 1, "w": 0x2001}, {"padded": 1, "xs": (1 << 23) + 16}):  # fmt: skip
+        assert linear(**{**tiled, **bad}) == -2, bad
+
+    def pad(m=2, n=20, qs=20, os=32, q=0x1000, out=0x2000):  # noqa: ANN001, ANN202
+        return lib.ts_int8_pad_rows(q, qs, out, os, m, n, None)
+
+    assert pad(m=0) == 0 and pad(n=0) == 0
+    for bad in ({"m": -1}, {"m": big}, {"n": big}, {"qs": -1}, {"os": 16}, {"os": 40}, {"out": 0x2008}, {"q": None}, {"out": None}):
+        assert pad(**bad) == -1, bad
 
     def embed(t=2, n=4, rows=5, ts=4, os=4, dtype=1, table=0x1000, scale=0x2000, ids=0x3000, out=0x4000):  # noqa: ANN001, ANN202
         return lib.ts_int8_embedding(table, ts, scale, rows, ids, out, os, t, n, dtype, None)
@@ -351,6 +362,20 @@ def test_linear_equals_the_definition(m: int, n: int, k: int, dtype: torch.dtype
     xa.copy_(x.q)
     wa.copy_(w.q)
     assert same(int8_linear(Int8Rows(xa, x.scale), Int8Rows(wa, w.scale), dtype).cpu(), got.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("m", "n"), [(4100, 4100), (2751, 6144), (1030, 4090), (520, 4100), (260, 1030), (129, 70)])
+def test_every_tile_shape_and_last_columns(m: int, n: int) -> None:
+    """Sizes that take each of the tile shapes, at column counts around their tiles of 128."""
+    for k in (1, 15, 16, 17, 112, 113, 127, 128, 129, 136, 144, 255, 256, 400, 515):
+        x = Int8Rows(codes(m, k, m + k, full=True).to(DEVICE), scales(m, m).to(DEVICE))
+        w = Int8Rows(codes(n, k, n - k, full=True).to(DEVICE), scales(n, n).to(DEVICE))
+        got = int8_linear(x, w, torch.float32)
+        acc = (x.q.float() @ w.q.float().t()) if k <= 1024 else None  # integers below 2^24: exact
+        assert same(got, acc * x.scale[:, None] * w.scale), k
+        half = int8_linear(x, w, torch.bfloat16)
+        assert same(half, (acc * x.scale[:, None] * w.scale).bfloat16()), k
 
 
 @pytest.mark.gpu

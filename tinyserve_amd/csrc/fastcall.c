@@ -104,8 +104,10 @@ ENTRY(ts_int8_quantize_rows, 14,
       P(0), P(1), P(2), P(3), P(4), I(5), I(6), L(7), L(8), L(9), F(10), I(11), I(12), P(13))
 ENTRY(ts_int8_embedding, 11,
       P(0), L(1), P(2), L(3), P(4), P(5), L(6), I(7), I(8), I(9), P(10))
-ENTRY(ts_int8_linear, 13,
-      P(0), L(1), P(2), P(3), L(4), P(5), P(6), L(7), I(8), I(9), I(10), I(11), P(12))
+ENTRY(ts_int8_linear, 14,
+      P(0), L(1), P(2), P(3), L(4), P(5), P(6), L(7), I(8), I(9), I(10), I(11), I(12), P(13))
+ENTRY(ts_int8_pad_rows, 7,
+      P(0), L(1), P(2), L(3), I(4), I(5), P(6))
 
 #define EACH(X)                                                                     \
   X(ts_decode_split)                                                                \
@@ -120,7 +122,8 @@ ENTRY(ts_int8_linear, 13,
   X(ts_add_rms_norm)                                                                \
   X(ts_int8_quantize_rows)                                                          \
   X(ts_int8_embedding)                                                              \
-  X(ts_int8_linear)
+  X(ts_int8_linear)                                                                 \
+  X(ts_int8_pad_rows)
 
 /* Whether an argument list's letters are `want`, letter for letter. */
 static int same_kinds(const char* kinds, const char* want) {

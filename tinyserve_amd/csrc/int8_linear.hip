@@ -14,6 +14,8 @@
 namespace ts {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4), may_alias));
+typedef u32x4 u32x4_alias __attribute__((may_alias));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 struct LinearArgs {
@@ -45,10 +47,11 @@ __device__ __forceinline__ i32x4 load_codes_tail(const int8_t* row, int k, int K
   return r.v;
 }
 
-template <typename T, int N>
-struct Loose {
-  typedef T Vec __attribute__((ext_vector_type(N)));
-  typedef Vec V __attribute__((aligned(1), may_alias));
+// Four outputs: at any address, and in LDS beside other types.
+template <typename T>
+struct Vec4 {
+  typedef T V __attribute__((ext_vector_type(4), may_alias));
+  typedef V Loose __attribute__((aligned(1)));
 };
 
 // Four outputs n .. n + 3 of row m.
@@ -57,10 +60,10 @@ __device__ __forceinline__ void store_outputs(const LinearArgs& a, int m, int n,
   const float s = a.xscale[m];
   T* o = static_cast<T*>(a.out) + m * a.os + n;
   if (n + 4 <= a.N) {
-    typename Loose<T, 4>::Vec y;
+    typename Vec4<T>::V y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(static_cast<float>(sum[i]) * s * a.wscale[n + i]);
-    *reinterpret_cast<typename Loose<T, 4>::V*>(o) = y;
+    *reinterpret_cast<typename Vec4<T>::Loose*>(o) = y;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -159,9 +162,8 @@ __global__ __launch_bounds__(KP * kWave) void int8_rows_kernel(const LinearArgs 
 
 template <typename T, int KP, int NTW, int MT>
 static int launch_rows8(const LinearArgs& a, hipStream_t st) {
-  const int64_t gx = (a.N + 16 * NTW - 1) / (16 * NTW), gy = (a.M + 16 * MT - 1) / (16 * MT);
-  if (gy > 65535) return TS_EUNSUPPORTED;
-  hipLaunchKernelGGL((int8_rows_kernel<T, KP, NTW, MT>), dim3(gx, gy), dim3(KP * kWave), 0, st, a);
+  hipLaunchKernelGGL((int8_rows_kernel<T, KP, NTW, MT>), dim3((a.N + 16 * NTW - 1) / (16 * NTW), (a.M + 16 * MT - 1) / (16 * MT)),
+                     dim3(KP * kWave), 0, st, a);
   return launch_status();
 }
 
@@ -169,29 +171,35 @@ static int launch_rows8(const LinearArgs& a, hipStream_t st) {
 // Each of the workgroup's GM x GN waves takes 32 MW rows of x and 32 NW rows of W: MW * NW
 // accumulators of v_mfma_i32_32x32x32_i8, W the A operand and x the B operand.
 //
-// Both operands go through a ring of kStages LDS tiles of 64 columns, filled by direct-to-LDS
-// loads (four lanes per row of 64 bytes) while older tiles are multiplied. Row r's 16-byte unit c
-// sits in slot c ^ swizzle(r), which spreads any 8 or 16 rows' units c over all banks; the lanes
-// of a load fetch the units that their slots hold. A step's operands are read from LDS while the
-// step before is multiplied; the barrier that hands over the next tile stands between a tile's
-// two steps, so the last product of one tile covers the first reads of the next.
+// Both operands go through a ring of kStages LDS tiles of kCols columns, filled by direct-to-LDS
+// loads (kCols / 16 lanes per row) while older tiles are multiplied. Row r's 16-byte unit c sits
+// in slot c ^ swizzle(r), which spreads any 8 or 16 rows' units c over all banks; the lanes of a
+// load fetch the units that their slots hold. A step's operands are read from LDS while the step
+// before is multiplied; the barrier that hands over the next tile stands before a tile's last
+// step, so that its product covers the first reads of the next.
 //
-// kAligned false: rows that do not start at multiples of 16 bytes go through registers instead
-// (unaligned vector loads), one tile ahead.
-//
-// The last K % 64 columns come first, alone, with zeros past the end of the rows.
-__device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+// Columns past the last whole tile: one more tile that ends where the rows (rounded up to 16
+// columns) end; the columns of it that the tile before held, or that lie past K, are masked out
+// of W's operand in registers.
+template <int kUnits>
+__device__ __forceinline__ int swizzle(int r) {
+  return (kUnits == 4 ? (r >> 1) & 3 : r & 7) ^ ((r >> 3) & 1);
+}
 
-template <typename T, int MW, int NW, int GM, int GN, int kStages, bool kAligned>
-__global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
+template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
+__global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
   constexpr int kWaves = GM * GN, kThreads = kWaves * kWave;
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
-  constexpr int kStage = (BM + BN) * 64;      // bytes: BN rows of W, then BM rows of x
-  constexpr int LPW = (BM + BN) / 16 / kWaves;  // loads per wave and tile, 16 rows each
+  constexpr int kUnits = kCols / 16, kSteps = kCols / 32, RPL = kWave / kUnits;  // RPL: rows per load
+  constexpr int kXTile = BM * kCols, kWTile = BN * kCols;  // bytes
+  constexpr int XL = BM / RPL / kWaves, WL = BN / RPL / kWaves;  // loads per wave and tile
   constexpr int kRow = 32 * NW * sizeof(T) + 16;  // bytes of a row of the output staging
-  constexpr int kLds = kStages * kStage > kWaves * 32 * kRow ? kStages * kStage : kWaves * 32 * kRow;
-  static_assert((BM + BN) % (16 * kWaves) == 0 && kLds <= 160 * 1024, "tile shape");
+  constexpr int kRing = kStages * (kXTile + kWTile), kStaged = kWaves * 32 * kRow + (BM + BN) * 4;
+  constexpr int kLds = kRing > kStaged ? kRing : kStaged;
+  static_assert(BM % (RPL * kWaves) == 0 && BN % (RPL * kWaves) == 0 && kLds <= 160 * 1024, "tile shape");
   __shared__ __attribute__((aligned(16))) int8_t lds[kLds];
+  int8_t* const x_ring = lds;
+  int8_t* const w_ring = lds + kStages * kXTile;
 
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -209,24 +217,35 @@ __global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const Linear
     tn = in / high;
   }
   const int m0 = tm * BM, n0 = tn * BN;
+  // Each thread keeps a few of the tile's scales until the end.
+  constexpr int kScales = (BM + BN + kThreads - 1) / kThreads;
+  float scale[kScales];
+#pragma unroll
+  for (int i = 0; i < kScales; ++i) {
+    const int c = threadIdx.x + i * kThreads;
+    scale[i] = c < BN ? a.wscale[min(n0 + c, a.N - 1)] : a.xscale[min(m0 + c - BN, a.M - 1)];
+  }
   const int8_t* wg = a.w + static_cast<int64_t>(n0) * a.ws;
   const int8_t* xg = a.x + static_cast<int64_t>(m0) * a.xs;
 
-  // Load j of this wave fills LDS rows 16 (wave * LPW + j) .. + 15, four lanes each; rows past the
-  // ends repeat the last one (their sums are not stored).
-  auto load_row = [&](int j) { return 16 * (wave * LPW + j) + lane / 4; };
-  const int load_unit = (lane % 4) ^ swizzle(lane / 4);
-  uint32_t off[LPW];
+  // Load j of this wave fills rows RPL (wave * XL + j) .. of an x tile (WL: of a W tile), kUnits
+  // lanes each; rows past the ends repeat the last one (their sums are not stored).
+  const int padded = (a.K + 15) & ~15;
+  auto x_row = [&](int j) { return RPL * (wave * XL + j) + lane / kUnits; };
+  auto w_row = [&](int j) { return RPL * (wave * WL + j) + lane / kUnits; };
+  auto column = [&](int r) { return min(((lane % kUnits) ^ swizzle<kUnits>(r)) * 16, padded - 16); };
+  uint32_t x_off[XL], w_off[WL];
 #pragma unroll
-  for (int j = 0; j < LPW; ++j) {
-    const int r = load_row(j);
-    const int64_t row = r < BN ? min(r, a.N - 1 - n0) * a.ws : min(r - BN, a.M - 1 - m0) * a.xs;
-    off[j] = static_cast<uint32_t>(row) + load_unit * 16;
-  }
+  for (int j = 0; j < XL; ++j)
+    x_off[j] = static_cast<uint32_t>(min(x_row(j), a.M - 1 - m0) * a.xs) + column(x_row(j));
+#pragma unroll
+  for (int j = 0; j < WL; ++j)
+    w_off[j] = static_cast<uint32_t>(min(w_row(j), a.N - 1 - n0) * a.ws) + column(w_row(j));
   // LDS bytes of unit 2 s + lane / 32 of row lane % 32 of a 32-row operand tile.
-  int unit[2];
+  int unit[kSteps];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) unit[s] = (lane % 32) * 64 + (((2 * s + lane / 32) ^ swizzle(lane % 32)) * 16);
+  for (int s = 0; s < kSteps; ++s)
+    unit[s] = (lane % 32) * kCols + (((2 * s + lane / 32) ^ swizzle<kUnits>(lane % 32)) * 16);
 
   i32x16 acc[NW][MW];
 #pragma unroll
@@ -236,90 +255,93 @@ __global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const Linear
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][u][i] = 0;
 
-  i32x4 wf[2][NW], xf[2][MW];  // operands of the two steps of a tile
-  auto read_w = [&](int s, int t, const int8_t* tile) {
-    wf[s][t] = *reinterpret_cast<const i32x4*>(tile + (wn * NW + t) * 2048 + unit[s]);
-  };
-  auto read_x = [&](int s, int u, const int8_t* tile) {
-    xf[s][u] = *reinterpret_cast<const i32x4*>(tile + BN * 64 + (wm * MW + u) * 2048 + unit[s]);
-  };
-  auto read_all = [&](int s, const int8_t* tile) {
+  i32x4 wf[2][NW], xf[2][MW];  // operands of two steps, taken in turn
+  auto read_all = [&](int s, const int8_t* xt, const int8_t* wt) {
 #pragma unroll
-    for (int t = 0; t < NW; ++t) read_w(s, t, tile);
+    for (int t = 0; t < NW; ++t) wf[s & 1][t] = *reinterpret_cast<const i32x4*>(wt + (wn * NW + t) * 32 * kCols + unit[s]);
 #pragma unroll
-    for (int u = 0; u < MW; ++u) read_x(s, u, tile);
+    for (int u = 0; u < MW; ++u) xf[s & 1][u] = *reinterpret_cast<const i32x4*>(xt + (wm * MW + u) * 32 * kCols + unit[s]);
   };
   auto multiply = [&](int s, int p) {  // product p of step s
-    acc[p / MW][p % MW] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s][p / MW], xf[s][p % MW], acc[p / MW][p % MW], 0, 0, 0);
+    acc[p / MW][p % MW] =
+        __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][p / MW], xf[s & 1][p % MW], acc[p / MW][p % MW], 0, 0, 0);
   };
   auto multiply_all = [&](int s) {
 #pragma unroll
     for (int p = 0; p < NW * MW; ++p) multiply(s, p);
   };
 
-  const int tiles = a.K / 64;
-  if (a.K % 64) {
+  const int whole = a.K / kCols, tiles = (a.K + kCols - 1) / kCols;
+  const int last = max(padded - kCols, 0);  // the last tile's first column
+  auto load_x = [&](int j, int kt, int8_t* tile) {
+    lds_load16_s(xg + min(kt * kCols, last), x_off[j], (TS_LDS void*)(tile + RPL * (wave * XL + j) * kCols));
+  };
+  auto load_w = [&](int j, int kt, int8_t* tile) {
+    lds_load16_s(wg + min(kt * kCols, last), w_off[j], (TS_LDS void*)(tile + RPL * (wave * WL + j) * kCols));
+  };
+  int slot = 0;
+  if (tiles > 0) {
+    for (int kt = 0; kt < min(kStages, tiles); ++kt) {
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-      const int r = load_row(j);
-      const int8_t* row = r < BN ? wg + min(r, a.N - 1 - n0) * a.ws : xg + min(r - BN, a.M - 1 - m0) * a.xs;
-      *reinterpret_cast<i32x4*>(lds + r * 64 + (lane % 4) * 16) = load_codes_tail(row, tiles * 64 + load_unit * 16, a.K);
+      for (int j = 0; j < XL; ++j) load_x(j, kt, x_ring + kt * kXTile);
+#pragma unroll
+      for (int j = 0; j < WL; ++j) load_w(j, kt, w_ring + kt * kWTile);
     }
-    __syncthreads();
-    read_all(0, lds);
-    read_all(1, lds);
-    multiply_all(0);
-    multiply_all(1);
-    __syncthreads();
-  }
-
-  if constexpr (kAligned) {
-    auto load = [&](int j, int kt, int8_t* tile) {
-      const int row0 = 16 * (wave * LPW + j);
-      const int8_t* base = (row0 < BN ? wg : xg) + static_cast<int64_t>(kt) * 64;
-      lds_load16_s(base, off[j], (TS_LDS void*)(tile + row0 * 64));
-    };
-    for (int kt = 0; kt < min(kStages, tiles); ++kt)
-#pragma unroll
-      for (int j = 0; j < LPW; ++j) load(j, kt, lds + kt * kStage);
-    if (tiles >= kStages) ring_barrier<(kStages - 1) * LPW>();
+    if (tiles >= kStages) ring_barrier<(kStages - 1) * (XL + WL)>();
     else ring_barrier<0>();
-    if (tiles > 0) read_all(0, lds);
-    int at = 0;  // LDS offset of tile kt
-    for (int kt = 0; kt < tiles; ++kt) {
-      int8_t* tile = lds + at;
-      at = at + kStage == kStages * kStage ? 0 : at + kStage;
-      int8_t* next = lds + at;
-      read_all(1, tile);
-      multiply_all(0);
-      // Every read of this tile is done and the next one has landed, in every wave.
-      if (kt + kStages - 1 < tiles) ring_barrier<(kStages - 2) * LPW>();
-      else ring_barrier<0>();
-      if (kt + kStages < tiles) {
+    read_all(0, x_ring, w_ring);
+    // Step s's products with loads of tile kt spread among them: issued together, they would hold
+    // up the wave's products for as long as the load path takes them in.
+    int8_t *x_free = x_ring, *w_free = w_ring;  // the slots that the last barrier freed
+    auto step = [&](int s, int xn, int wn, int kt) {
+      constexpr int P = NW * MW;
 #pragma unroll
-        for (int j = 0; j < LPW; ++j) load(j, kt + kStages, tile);
+      for (int p = 0; p < P; ++p) {
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, p);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt >= tiles) continue;
+#pragma unroll
+        for (int j = 0; j < xn; ++j)
+          if (j * P / xn == p) load_x(j, kt, x_free);
+#pragma unroll
+        for (int j = 0; j < wn; ++j)
+          if (j * P / wn == p) load_w(j, kt, w_free);
       }
-      if (kt + 1 < tiles) read_all(0, next);
-      multiply_all(1);
-    }
-  } else if (tiles > 0) {
-    i32x4 held[LPW];
-    auto fetch = [&](int kt) {
-#pragma unroll
-      for (int j = 0; j < LPW; ++j)
-        held[j] = load_codes((16 * (wave * LPW + j) < BN ? wg : xg) + static_cast<int64_t>(kt) * 64 + off[j]);
+      __builtin_amdgcn_sched_barrier(0);
     };
-    fetch(0);
-    for (int kt = 0; kt < tiles; ++kt) {
-      int8_t* tile = lds + (kt & 1) * kStage;
+    for (int kt = 0; kt < whole; ++kt) {
+      int8_t *xt = x_ring + slot * kXTile, *wt = w_ring + slot * kWTile;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
 #pragma unroll
-      for (int j = 0; j < LPW; ++j) *reinterpret_cast<i32x4*>(tile + load_row(j) * 64 + (lane % 4) * 16) = held[j];
-      if (kt + 1 < tiles) fetch(kt + 1);
-      __syncthreads();  // two tiles: the one before this is read by no wave that has passed it
-      read_all(0, tile);
-      read_all(1, tile);
-      multiply_all(0);
-      multiply_all(1);
+      for (int s = 0; s + 1 < kSteps; ++s) {
+        read_all(s + 1, xt, wt);
+        step(s, 0, s == 0 ? WL : 0, kt > 0 ? kt - 1 + kStages : tiles);
+      }
+      // Every read of this tile is done and the next one has landed, in every wave.
+      if (kt + kStages - 1 < tiles) ring_barrier<(kStages - 2) * (XL + WL)>();
+      else ring_barrier<0>();
+      x_free = xt;
+      w_free = wt;
+      if (kt + 1 < tiles) read_all(0, x_ring + slot * kXTile, w_ring + slot * kWTile);
+      step(kSteps - 1, XL, 0, kt + kStages);
+    }
+    if (whole < tiles) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int col = last + (2 * s + lane / 32) * 16;
+        const int valid = col < whole * kCols ? 0 : a.K - col;  // bytes of this lane's unit
+        i32x4 mask;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int bytes = valid - 4 * d;
+          mask[d] = bytes >= 4 ? -1 : bytes <= 0 ? 0 : (1 << (8 * bytes)) - 1;
+        }
+#pragma unroll
+        for (int t = 0; t < NW; ++t) wf[s & 1][t] &= mask;
+        if (s + 1 < kSteps) read_all(s + 1, x_ring + slot * kXTile, w_ring + slot * kWTile);
+        multiply_all(s);
+      }
     }
   }
   __syncthreads();  // the ring's last reads, before the outputs take its place
@@ -327,29 +349,33 @@ __global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const Linear
   // Lane l holds column l % 32 (a row of x) and rows 8 j + 4 (l / 32) .. + 3 (of W) of each result.
   // 32 rows of outputs at a time go through the wave's own part of LDS and out in whole vectors.
   int8_t* mine = lds + wave * 32 * kRow;
+  float* scales = reinterpret_cast<float*>(lds + kWaves * 32 * kRow);  // of BN rows of W, then BM of x
+#pragma unroll
+  for (int i = 0; i < kScales; ++i)
+    if (threadIdx.x + i * kThreads < BM + BN) scales[threadIdx.x + i * kThreads] = scale[i];
+  __syncthreads();
   constexpr int E = Pack16<T>::N, VPR = 32 * NW / E;  // vectors per row
 #pragma unroll
   for (int u = 0; u < MW; ++u) {
-    const int mrow = m0 + (wm * MW + u) * 32;
-    const float s = a.xscale[min(mrow + lane % 32, a.M - 1)];
+    const float s = scales[BN + (wm * MW + u) * 32 + lane % 32];
 #pragma unroll
     for (int t = 0; t < NW; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = t * 32 + j * 8 + lane / 32 * 4;
-        const int n = n0 + wn * 32 * NW + c;
-        typename Loose<T, 4>::Vec y;
+        const f32x4 sw = *reinterpret_cast<const f32x4*>(scales + wn * 32 * NW + c);
+        typename Vec4<T>::V y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          y[i] = from_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * a.wscale[min(n + i, a.N - 1)]);
-        *reinterpret_cast<typename Loose<T, 4>::Vec*>(mine + (lane % 32) * kRow + c * sizeof(T)) = y;
+        for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * sw[i]);
+        *reinterpret_cast<typename Vec4<T>::V*>(mine + (lane % 32) * kRow + c * sizeof(T)) = y;
       }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int v = 0; v < 32 * VPR / kWave; ++v) {
       const int r = (v * kWave + lane) / VPR, c = (v * kWave + lane) % VPR * E;
-      const int m = mrow + r, n = n0 + wn * 32 * NW + c;
-      const Pack16<T> y = load16(reinterpret_cast<const T*>(mine + r * kRow) + c);
+      const int m = m0 + (wm * MW + u) * 32 + r, n = n0 + wn * 32 * NW + c;
+      Pack16<T> y;
+      y.raw = *reinterpret_cast<const u32x4_alias*>(mine + r * kRow + c * sizeof(T));
       if (m >= a.M) continue;
       T* o = static_cast<T*>(a.out) + m * a.os + n;
       if (n + E <= a.N) {
@@ -364,26 +390,72 @@ __global__ __launch_bounds__(GM * GN * kWave) void int8_tile_kernel(const Linear
   }
 }
 
-template <typename T, int MW, int NW, int GM, int GN, int kStages, bool kAligned>
+template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
 static int launch_tiles(const LinearArgs& a, hipStream_t st) {
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
   const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
   if (tm * tn > INT32_MAX) return TS_EUNSUPPORTED;
-  hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kStages, kAligned>), dim3(static_cast<unsigned>(tm * tn)),
+  hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kCols, kStages>), dim3(static_cast<unsigned>(tm * tn)),
                      dim3(GM * GN * kWave), 0, st, a, static_cast<int>(tm), static_cast<int>(tn));
   return launch_status();
 }
 
+// Tile shapes, and what a tile of each takes on a compute unit: a fixed part (launch, the ring's
+// first fill, outputs) and a part per 1024 columns, in us as fitted to captured launches. The
+// chip takes ceil(tiles / CUs) of them one after another, so large tiles (fewer LDS reads per
+// product) pay where there are many of them and small ones where there are few. Measured (us, in
+// the order of the table): 8192 x 8192 x 8192 452, 502, 620, 694, 851; 2751 x 6144 x 1024 35.2,
+// 28.8, 35.2, 34.1, 41.2; 1024 x 4096 x 4096 41.9, 29.9, 22.9, 25.2, 30.5; 512 x 4096 x 1024
+// 16.0, 11.4, 8.5, 7.2, 7.7; 256 x 1024 x 2048 23.9, 16.3, 10.6, 8.9, 7.0.
+struct TileShape {
+  int bm, bn;
+  float fixed, per_k;
+};
+constexpr int kRowsMax = 128;  // more rows go through tiles
+constexpr TileShape kShapes[] = {
+    {256, 256, 6.4f, 10.1f},  // 8 waves of 128 x 64
+    {192, 128, 3.6f, 5.0f},   // 4 waves of 96 x 64, two workgroups per CU
+    {128, 128, 2.2f, 4.4f},   // 8 waves of 64 x 32, three stages
+    {64, 128, 1.3f, 2.3f},    // 4 waves of 32 x 64, three stages, two workgroups per CU
+    {64, 64, 1.0f, 1.6f},     // 4 waves of 32 x 32, four stages, two workgroups per CU
+};
+
+static int pick_shape(int M, int N, int K) {
+  const int cus = compute_units();
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 5; ++i) {
+    const TileShape& t = kShapes[i];
+    const int64_t tiles = static_cast<int64_t>((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const float us = static_cast<float>((tiles + cus - 1) / cus) * (t.fixed + t.per_k * static_cast<float>(K) / 1024.f);
+    if (i == 0 || us < least) {
+      best = i;
+      least = us;
+    }
+  }
+  return best;
+}
+
+// Rows that tiles take: 16-byte aligned, readable to a whole 16 columns, and, as rows are addressed
+// by 32-bit offsets, at most 2^23 bytes apart.
+static bool tiles_fit(const LinearArgs& a, bool padded) {
+  const int64_t at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w)) | a.xs | a.ws;
+  return at % 16 == 0 && (padded || a.K % 16 == 0) && a.xs <= 1 << 23 && a.ws <= 1 << 23;
+}
+
 template <typename T>
-static int launch_linear(const LinearArgs& a, hipStream_t st) {
+static int launch_linear(const LinearArgs& a, bool padded, hipStream_t st) {
   if (a.M <= 16) return launch_rows8<T, 8, 1, 1>(a, st);
   if (a.M <= 32) return launch_rows8<T, 8, 1, 2>(a, st);
-  // Tiles address their rows by 32-bit offsets: 255 rows of at most 2^23 bytes.
-  if (a.M <= 128 || a.xs > 1 << 23 || a.ws > 1 << 23) return launch_rows8<T, 8, 1, 4>(a, st);
-  const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.xs | a.ws) & 15) == 0;
-  if (!aligned) return launch_tiles<T, 2, 2, 2, 2, 2, false>(a, st);
-  if (a.M >= 1024 && a.N >= 1024) return launch_tiles<T, 4, 4, 2, 2, 4, true>(a, st);
-  return launch_tiles<T, 2, 2, 2, 2, 4, true>(a, st);
+  if (a.M <= kRowsMax) return launch_rows8<T, 8, 1, 4>(a, st);
+  if (!tiles_fit(a, padded)) return TS_EUNSUPPORTED;
+  switch (pick_shape(a.M, a.N, a.K)) {
+    case 0: return launch_tiles<T, 4, 2, 2, 4, 128, 2>(a, st);
+    case 1: return launch_tiles<T, 3, 2, 2, 2, 128, 2>(a, st);
+    case 2: return launch_tiles<T, 2, 1, 2, 4, 128, 3>(a, st);
+    case 3: return launch_tiles<T, 1, 2, 2, 2, 128, 3>(a, st);
+    default: return launch_tiles<T, 1, 1, 2, 2, 128, 4>(a, st);
+  }
 }
 
 }  // namespace ts
@@ -391,8 +463,8 @@ static int launch_linear(const LinearArgs& a, hipStream_t st) {
 using namespace ts;
 
 extern "C" int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
-                              const float* w_scale, void* out, int64_t o_stride, int M, int N, int K, int dtype,
-                              void* stream) {
+                              const float* w_scale, void* out, int64_t o_stride, int M, int N, int K, int padded,
+                              int dtype, void* stream) {
   if (M < 0 || M > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM || K < 0 || K > TS_INT8_MAX_K || x_stride < 0 || w_stride < 0) return TS_EINVAL;
   if (M > 1 && o_stride < N) return TS_EINVAL;
   if (dtype < TS_F32 || dtype > TS_BF16) return TS_EUNSUPPORTED;
@@ -401,8 +473,8 @@ extern "C" int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_
   const LinearArgs a{x, w, x_scale, w_scale, out, M, N, K, x_stride, w_stride, o_stride};
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case TS_F32: return launch_linear<float>(a, st);
-    case TS_F16: return launch_linear<f16>(a, st);
-    default: return launch_linear<bf16>(a, st);
+    case TS_F32: return launch_linear<float>(a, padded != 0, st);
+    case TS_F16: return launch_linear<f16>(a, padded != 0, st);
+    default: return launch_linear<bf16>(a, padded != 0, st);
   }
 }

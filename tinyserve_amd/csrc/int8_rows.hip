@@ -331,6 +331,30 @@ __global__ __launch_bounds__(256) void int8_embedding_kernel(const int8_t* __res
   }
 }
 
+// Rows copied to a stride of whole 16 bytes, zeros past their ends. One thread per 16 bytes.
+__global__ __launch_bounds__(256) void int8_pad_rows_kernel(const int8_t* __restrict__ q, int64_t qs, int8_t* __restrict__ out,
+                                                            int64_t os, int rows, int N, int per_row) {
+  const int64_t total = static_cast<int64_t>(rows) * per_row;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t t = u / per_row;
+    const int i = static_cast<int>(u - t * per_row) * 16;
+    const int8_t* p = q + t * qs + i;
+    union {
+      u32x4 raw;
+      int8_t b[16];
+    } c;
+    c.raw = u32x4{0, 0, 0, 0};
+    if (i + 16 <= N) {
+      c.raw = load16_loose(p).raw;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (i + e < N) c.b[e] = p[e];
+    }
+    *reinterpret_cast<u32x4*>(out + t * os + i) = c.raw;
+  }
+}
+
 template <typename T>
 static int launch_embedding(const int8_t* q, int64_t qs, const float* scale, int64_t table, const int64_t* ids, void* out,
                             int64_t os, int rows, int N, hipStream_t st) {
@@ -389,4 +413,17 @@ extern "C" int ts_int8_embedding(const int8_t* table, int64_t t_stride, const fl
     case TS_F16: return launch_embedding<f16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
     default: return launch_embedding<bf16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
   }
+}
+
+extern "C" int ts_int8_pad_rows(const int8_t* q, int64_t q_stride, int8_t* out, int64_t o_stride, int M, int N, void* stream) {
+  const int64_t padded = (static_cast<int64_t>(N) + 15) / 16 * 16;
+  if (M < 0 || M > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM || q_stride < 0) return TS_EINVAL;
+  if (o_stride < padded || o_stride % 16 || reinterpret_cast<uintptr_t>(out) % 16) return TS_EINVAL;
+  if (M == 0 || N == 0) return 0;
+  if (!q || !out) return TS_EINVAL;
+  const int per_row = static_cast<int>(padded / 16);
+  const int64_t blocks = (static_cast<int64_t>(M) * per_row + 255) / 256;
+  hipLaunchKernelGGL(int8_pad_rows_kernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), q, q_stride, out, o_stride, M, N, per_row);
+  return launch_status();
 }

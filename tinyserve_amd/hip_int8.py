@@ -31,6 +31,7 @@ from tinyserve_amd import _lib
 PLAIN, NORM, ADD_NORM, SILU = 0, 1, 2, 3
 MAX_K = 131071  # products of longer rows could pass an int32
 MAX_DIM = 1 << 30  # rows or columns of one call
+ROWS_MAX, MAX_STRIDE = 128, 1 << 23  # of ts_int8_linear: rows read as they are, and bytes between tiled ones
 
 
 class Int8Rows(NamedTuple):
@@ -48,6 +49,21 @@ def _call(dev: int, name: str, *args: object) -> None:
     else:
         with torch.cuda.device(dev):
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _aligned(q: torch.Tensor) -> bool:
+    """Whether rows start at multiples of 16 bytes and may be read to a whole 16 columns."""
+    m, k = q.shape
+    return (q.data_ptr() % 16 == 0 and q.stride(0) % 16 == 0 and
+            (k % 16 == 0 or q.storage_offset() + (m - 1) * q.stride(0) + (k + 15) // 16 * 16 <= q.untyped_storage().nbytes()))  # fmt: skip
+
+
+def _padded(q: torch.Tensor, dev: int) -> torch.Tensor:
+    """A copy of ``q`` whose rows are 16-byte aligned and padded with zeros."""
+    m, k = q.shape
+    out = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=q.device)
+    _call(dev, "ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k)
+    return out
 
 
 def _check_matrix(x: torch.Tensor, what: str) -> None:
@@ -142,8 +158,8 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
 
     Args:
         x: ``[M, K]`` tokens. w: ``[N, K]`` weights, a scale per output channel. K up to 131071;
-            rows that start at multiples of 16 bytes, as the functions here make them, are
-            read fastest.
+            over 128 tokens, rows that do not start at multiples of 16 bytes (the functions
+            here make them so) are copied first.
         out: ``[M, N]`` in ``dtype``, unit column stride (default: a new tensor).
     """
     xq, xs = x
@@ -168,8 +184,13 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
         if _lib.require_device(out) != dev:
             raise ValueError("out is on another device")
     if m and n:
+        if m > ROWS_MAX:  # read in tiles: rows that are not 16-byte aligned are copied first
+            if not _aligned(xq) or xq.stride(0) > MAX_STRIDE:
+                xq = _padded(xq, dev)
+            if not _aligned(wq) or wq.stride(0) > MAX_STRIDE:
+                wq = _padded(wq, dev)
         _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-              ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, code)  # fmt: skip
+              ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, int(m > ROWS_MAX), code)  # fmt: skip
     return out
 
 
