@@ -332,11 +332,12 @@ int ts_int8_embedding(const int8_t* table, int64_t t_stride, const float* scale,
  * out[m, n] = (dtype)((float)(sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n]): the product of
  * 8-bit rows x [M, K] and W [N, K] with a scale for each token and each channel. The int32 sums
  * are exact, so out does not depend on how the work is split. K at most TS_INT8_MAX_K; K == 0
- * multiplies zero by the scales. Up to 128 rows of x take any strides and alignment; more need x
- * and W 16-byte aligned, with strides that are multiples of 16 up to 2^23, and, where K is not a
- * multiple of 16, `padded` non-zero: the caller's word that every row may be read up to K rounded
- * up to 16 (those bytes do not count). Else TS_EUNSUPPORTED: ts_int8_pad_rows makes such rows. No
- * counterpart in the reference's kernels (F.linear of the decoder layer, model.py:137-179).
+ * multiplies zero by the scales. Rows are read fastest where x and W are 16-byte aligned, their
+ * strides multiples of 16 up to 2^23, and, where K is not a multiple of 16, `padded` non-zero: the
+ * caller's word that every row may be read up to K rounded up to 16 (those bytes do not count).
+ * Other rows are taken too where the output is small; at sizes that run in tiles they return
+ * TS_EUNSUPPORTED before any launch, and ts_int8_pad_rows makes rows that fit. No counterpart in
+ * the reference's kernels (F.linear of the decoder layer, model.py:137-179).
  */
 #define TS_INT8_MAX_K 131071
 int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w,

@@ -191,7 +191,7 @@ def test_c_abi_refuses_before_any_launch() -> None:
                 {"x": None}, {"w": None}, {"out": None}, {"a": None}, {"b": None}):  # fmt: skip
         assert linear(**bad) == -1, bad
     assert linear(dtype=7) == -2
-    tiled = {"m": 200, "k": 20, "xs": 32, "ws": 32}  # many rows: aligned and readable to 32 columns, or not taken
+    tiled = {"m": 4000, "n": 4000, "os": 4000, "k": 20, "xs": 32, "ws": 32}  # many rows: aligned and readable to 32 columns, or not taken
     for bad in ({"padded": 0}, {"padded": 1, "xs": 20}, {"padded": 1, "ws": 24}, {"padded": 1, "x": 0x1008},
                 {"padded": 1, "w": 0x2001}, {"padded": 1, "xs": (1 << 23) + 16}):  # fmt: skip
         assert linear(**{**tiled, **bad}) == -2, bad

@@ -71,27 +71,90 @@ __device__ __forceinline__ void store_outputs(const LinearArgs& a, int m, int n,
   }
 }
 
-// ---- few rows: W streamed through registers ---------------------------------------------------
-// A workgroup takes 16 * NTW rows of W and 16 * MT rows of x. Its KP waves take 128-column units
-// of K in turn, so that the waves side by side read whole lines of W; W is the A operand of
-// v_mfma_i32_16x16x64_i8 and x its B operand, both straight from global memory (16 codes per
-// lane: row l % 16, columns 16 (l / 16) .. + 15 of each 64). The waves' sums meet in LDS.
-template <typename T, int KP, int NTW, int MT>
-__global__ __launch_bounds__(KP * kWave) void int8_rows_kernel(const LinearArgs a) {
-  constexpr int BN = 16 * NTW, BM = 16 * MT;
-  constexpr int RED = BN + 4;  // padded row of the part sums, 16-byte aligned
-  __shared__ int red[KP > 1 ? KP * BM * RED : 1];
-  const int tid = threadIdx.x, lane = tid % kWave, kp = tid / kWave;
-  const int r16 = lane % 16, kq = lane / 16 * 16;
-  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
+// ---- few rows: the waves of a workgroup along K ------------------------------------------------
+// A workgroup takes 16 NTW rows of W and 16 MT rows of x; its KP waves take 128-column units of K
+// in turn, and their sums meet in LDS at the end. Each wave brings its own units into its own part
+// of LDS (direct-to-LDS loads, eight lanes per row, so that whole lines of W and x are asked for
+// once) and reads them back as operands of v_mfma_i32_16x16x64_i8, W the A operand: lane l holds
+// row l % 16, columns 16 (l / 16) .. + 15 of each 64. No wave waits for another before the end; as
+// soon as a unit is in registers, the loads of the next take its place. (Two or four units in
+// flight per wave leave room for fewer workgroups: 64 x 1024 x 2048 3.9 us, 32 x 8192 x 8192 21.4
+// against 18.4.)
+//
+// Loaded straight into operand registers, 16 rows at a time, each load takes about four times as
+// long (16 rows of 64 bytes, a row's lanes apart, instead of 8 of 128): M x N x K of 64 x 1024 x
+// 2048 7.3 us against 3.7, 64 x 4096 x 1024 5.9 against 4.6, 1 x 4096 x 1024 4.0 against 3.8.
+//
+// kAligned false: rows that are not 16-byte aligned, or are far apart, pass through registers on
+// their way (unaligned vector loads).
+template <int kUnits>
+__device__ __forceinline__ int swizzle(int r) {
+  return (kUnits == 4 ? (r >> 1) & 3 : r & 7) ^ ((r >> 3) & 1);
+}
 
-  // Rows past the ends repeat the last one: their sums are not stored.
-  const int8_t* wp[NTW];
-  const int8_t* xp[MT];
+// Wait for this wave's vector-memory loads.
+__device__ __forceinline__ void wait_loads() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Wait for this wave's LDS operations.
+__device__ __forceinline__ void wait_lds() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// The bytes lo .. hi - 1 of a 16-byte unit.
+__device__ __forceinline__ i32x4 byte_mask(int lo, int hi) {
+  auto below = [](int n) { return n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1; };
+  i32x4 m;
 #pragma unroll
-  for (int t = 0; t < NTW; ++t) wp[t] = a.w + static_cast<int64_t>(min(n0 + t * 16 + r16, a.N - 1)) * a.ws;
+  for (int d = 0; d < 4; ++d) m[d] = below(hi - 4 * d) & ~below(lo - 4 * d);
+  return m;
+}
+
+template <typename T, int NTW, int MT, bool kAligned>
+__global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a) {
+  constexpr int KP = 8, BN = 16 * NTW, BM = 16 * MT, L = (BM + BN) / 8;  // L: loads per unit
+  constexpr int RED = BN + 4;  // padded row of the part sums, 16-byte aligned
+  constexpr int kUnit = (BM + BN) * 128, kRing = KP * kUnit, kSums = KP * BM * RED * 4;
+  __shared__ __attribute__((aligned(16))) int8_t lds[kRing > kSums ? kRing : kSums];
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int kp = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
+  int8_t* const slot = lds + kp * kUnit;
+
+  // Load j fills rows 8 j .. of a unit, of W and then of x; rows past the ends repeat the last one
+  // (their sums are not stored). Unit row r's 16 columns c sit in slot c ^ swizzle(r).
+  const int units = a.K / 128, total = (a.K + 127) / 128;
+  const int padded = (a.K + 15) & ~15;
+  const int last = kAligned ? max(padded - 128, 0) : max(a.K - 128, 0);  // the last unit's first column
+  auto row_at = [&](int j) {
+    const int r = 8 * j + lane / 8;
+    return r < BN ? static_cast<int64_t>(min(r, a.N - 1 - n0)) * a.ws : static_cast<int64_t>(min(r - BN, a.M - 1 - m0)) * a.xs;
+  };
+  auto column = [&](int j) { return ((lane % 8) ^ swizzle<8>(8 * j + lane / 8)) * 16; };
+  const int8_t* wg = a.w + static_cast<int64_t>(n0) * a.ws;
+  const int8_t* xg = a.x + static_cast<int64_t>(m0) * a.xs;
+  uint32_t off[kAligned ? L : 1];
+  const int8_t* from[kAligned ? 1 : L];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xp[t] = a.x + static_cast<int64_t>(min(m0 + t * 16 + r16, a.M - 1)) * a.xs;
+  for (int j = 0; j < L; ++j) {
+    if constexpr (kAligned) off[j] = static_cast<uint32_t>(row_at(j)) + min(column(j), padded - 16);
+    else from[j] = (8 * j < BN ? wg : xg) + row_at(j);
+  }
+  i32x4 held[kAligned ? 1 : L];
+  auto fetch = [&](int u) {
+    const int k0 = min(u * 128, last);
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      if constexpr (kAligned) lds_load16_s((8 * j < BN ? wg : xg) + k0, off[j], (TS_LDS void*)(slot + j * 1024));
+      else if (a.K >= 128) held[j] = load_codes(from[j] + k0 + column(j));
+      else held[j] = load_codes_tail(from[j], column(j), a.K);
+    }
+  };
 
   i32x4 acc[NTW][MT];
 #pragma unroll
@@ -99,71 +162,71 @@ __global__ __launch_bounds__(KP * kWave) void int8_rows_kernel(const LinearArgs 
 #pragma unroll
     for (int u = 0; u < MT; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
 
-  i32x4 wv[2][NTW], xv[2][MT];
-  auto multiply = [&]() {
+  if (kp < total) fetch(kp);
+  for (int u = kp; u < total; u += KP) {
+    if constexpr (kAligned) {
+      wait_loads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < L; ++j) *reinterpret_cast<i32x4*>(slot + j * 1024 + lane * 16) = held[j];
+      if (u + KP < total) fetch(u + KP);
+      wait_lds();
+    }
+    i32x4 wv[2][NTW], xv[2][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int8_t* p = slot + (lane % 16) * 128 + (((4 * s + lane / 16) ^ swizzle<8>(lane % 16)) * 16);
+#pragma unroll
+      for (int t = 0; t < NTW; ++t) wv[s][t] = *reinterpret_cast<const i32x4*>(p + t * 2048);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xv[s][t] = *reinterpret_cast<const i32x4*>(p + (NTW + t) * 2048);
+    }
+    wait_lds();  // the unit is in registers: its slot is free
+    if constexpr (kAligned)
+      if (u + KP < total) fetch(u + KP);
+    if (u == units) {  // the last, partial unit: W's columns of the unit before and past K
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int col = last + (4 * s + lane / 16) * 16;
+        const i32x4 m = byte_mask(units * 128 - col, a.K - col);
+#pragma unroll
+        for (int t = 0; t < NTW; ++t) wv[s][t] &= m;
+      }
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int t = 0; t < NTW; ++t)
 #pragma unroll
-        for (int u = 0; u < MT; ++u) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[s][t], xv[s][u], acc[t][u], 0, 0, 0);
-  };
-  const int units = a.K / 128;
-  for (int u = kp; u < units; u += KP) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int k = u * 128 + s * 64 + kq;
-#pragma unroll
-      for (int t = 0; t < NTW; ++t) wv[s][t] = load_codes(wp[t] + k);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) xv[s][t] = load_codes(xp[t] + k);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // every load is issued before the first product
-    multiply();
+        for (int m = 0; m < MT; ++m)
+          acc[t][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[s][t], xv[s][m], acc[t][m], 0, 0, 0);
   }
-  if (a.K % 128 && units % KP == kp) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int k = units * 128 + s * 64 + kq;
-#pragma unroll
-      for (int t = 0; t < NTW; ++t) wv[s][t] = load_codes_tail(wp[t], k, a.K);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) xv[s][t] = load_codes_tail(xp[t], k, a.K);
-    }
-    multiply();
-  }
+  __syncthreads();  // every wave's units are in registers: the sums take their place
 
   // Lane l holds column l % 16 (a row of x) and rows 4 (l / 16) .. + 3 (of W) of each result.
-  if constexpr (KP == 1) {
+  int* red = reinterpret_cast<int*>(lds);
 #pragma unroll
-    for (int t = 0; t < NTW; ++t)
+  for (int t = 0; t < NTW; ++t)
 #pragma unroll
-      for (int u = 0; u < MT; ++u) {
-        const int m = m0 + u * 16 + r16, n = n0 + t * 16 + lane / 16 * 4;
-        if (m < a.M && n < a.N) store_outputs<T>(a, m, n, acc[t][u]);
-      }
-  } else {
+    for (int u = 0; u < MT; ++u)
+      *reinterpret_cast<i32x4*>(&red[(kp * BM + u * 16 + lane % 16) * RED + t * 16 + lane / 16 * 4]) = acc[t][u];
+  __syncthreads();
+  for (int i = tid; i < BM * (BN / 4); i += KP * kWave) {
+    const int m = i / (BN / 4), j = i % (BN / 4) * 4;
+    if (m0 + m >= a.M || n0 + j >= a.N) continue;
+    i32x4 v = {0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < NTW; ++t)
-#pragma unroll
-      for (int u = 0; u < MT; ++u)
-        *reinterpret_cast<i32x4*>(&red[(kp * BM + u * 16 + r16) * RED + t * 16 + lane / 16 * 4]) = acc[t][u];
-    __syncthreads();
-    for (int i = tid; i < BM * (BN / 4); i += KP * kWave) {
-      const int m = i / (BN / 4), j = i % (BN / 4) * 4;
-      if (m0 + m >= a.M || n0 + j >= a.N) continue;
-      i32x4 v = {0, 0, 0, 0};
-#pragma unroll
-      for (int p = 0; p < KP; ++p) v += *reinterpret_cast<const i32x4*>(&red[(p * BM + m) * RED + j]);
-      store_outputs<T>(a, m0 + m, n0 + j, v);
-    }
+    for (int p = 0; p < KP; ++p) v += *reinterpret_cast<const i32x4*>(&red[(p * BM + m) * RED + j]);
+    store_outputs<T>(a, m0 + m, n0 + j, v);
   }
 }
 
-template <typename T, int KP, int NTW, int MT>
-static int launch_rows8(const LinearArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((int8_rows_kernel<T, KP, NTW, MT>), dim3((a.N + 16 * NTW - 1) / (16 * NTW), (a.M + 16 * MT - 1) / (16 * MT)),
-                     dim3(KP * kWave), 0, st, a);
+template <typename T, int NTW, int MT>
+static int launch_rows8(const LinearArgs& a, bool aligned, hipStream_t st) {
+  const dim3 grid((a.N + 16 * NTW - 1) / (16 * NTW), (a.M + 16 * MT - 1) / (16 * MT)), block(8 * kWave);
+  if (grid.y > 65535) return TS_EUNSUPPORTED;
+  if (aligned) hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, false>), grid, block, 0, st, a);
   return launch_status();
 }
 
@@ -181,11 +244,6 @@ static int launch_rows8(const LinearArgs& a, hipStream_t st) {
 // Columns past the last whole tile: one more tile that ends where the rows (rounded up to 16
 // columns) end; the columns of it that the tile before held, or that lie past K, are masked out
 // of W's operand in registers.
-template <int kUnits>
-__device__ __forceinline__ int swizzle(int r) {
-  return (kUnits == 4 ? (r >> 1) & 3 : r & 7) ^ ((r >> 3) & 1);
-}
-
 template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
 __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
   constexpr int kWaves = GM * GN, kThreads = kWaves * kWave;
@@ -330,13 +388,7 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int col = last + (2 * s + lane / 32) * 16;
-        const int valid = col < whole * kCols ? 0 : a.K - col;  // bytes of this lane's unit
-        i32x4 mask;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const int bytes = valid - 4 * d;
-          mask[d] = bytes >= 4 ? -1 : bytes <= 0 ? 0 : (1 << (8 * bytes)) - 1;
-        }
+        const i32x4 mask = byte_mask(whole * kCols - col, a.K - col);
 #pragma unroll
         for (int t = 0; t < NW; ++t) wf[s & 1][t] &= mask;
         if (s + 1 < kSteps) read_all(s + 1, x_ring + slot * kXTile, w_ring + slot * kWTile);
@@ -411,7 +463,6 @@ struct TileShape {
   int bm, bn;
   float fixed, per_k;
 };
-constexpr int kRowsMax = 128;  // more rows go through tiles
 constexpr TileShape kShapes[] = {
     {256, 256, 6.4f, 10.1f},  // 8 waves of 128 x 64
     {192, 128, 3.6f, 5.0f},   // 4 waves of 96 x 64, two workgroups per CU
@@ -420,36 +471,73 @@ constexpr TileShape kShapes[] = {
     {64, 64, 1.0f, 1.6f},     // 4 waves of 32 x 32, four stages, two workgroups per CU
 };
 
-static int pick_shape(int M, int N, int K) {
+// Row kernels, as 16-row tiles of W and of x per workgroup, with what a workgroup takes beside its
+// loads (sums, outputs), in us.
+struct RowShape {
+  int ntw, mt;
+  float fixed;
+};
+constexpr RowShape kRowShapes[] = {{1, 1, 0.2f}, {2, 1, 0.3f}, {2, 2, 0.5f}, {4, 1, 0.5f}, {4, 2, 1.2f}, {4, 4, 2.5f}};
+
+// Which kernel: a tile shape (0 ..), or a row shape (-1 - index). Both are priced in us. A row
+// kernel takes, beside its start, what its workgroups bring into one compute unit, at about 50
+// KB a us (measured at 64 x 8192 x 8192, in the order of the
+// table but for the second: 41.8, 27.7, 26.8, 21.2, 26.7 us, and at 64 x 4096 x 1024 5.2, 4.6,
+// 4.7, 5.2, 6.5). Tiles that do not fill the chip wait for W: half as much again per column.
+// Measured, row kernel against tiles: 128 x 2048 x 4096 6.7 and 10.6, 64 x 8192 x 8192 21.2 and
+// 26.7, 128 x 8192 x 8192 25.6 and 26.4, 64 x 16384 x 2048 11.8 and 9.6, 64 x 151936 x 1024 62 and 35.
+static int pick_kernel(int M, int N, int K) {
   const int cus = compute_units();
+  const float k = static_cast<float>(K) / 1024.f;
+  auto times = [&](int bm, int bn) {  // workgroups per compute unit, one after another
+    const int64_t groups = static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    return static_cast<float>((groups + cus - 1) / cus);
+  };
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 5; ++i) {
     const TileShape& t = kShapes[i];
-    const int64_t tiles = static_cast<int64_t>((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-    const float us = static_cast<float>((tiles + cus - 1) / cus) * (t.fixed + t.per_k * static_cast<float>(K) / 1024.f);
+    const float us = times(t.bm, t.bn) * (t.fixed + t.per_k * k);
     if (i == 0 || us < least) {
       best = i;
       least = us;
     }
   }
-  return best;
+  const TileShape& t = kShapes[best];
+  if (static_cast<int64_t>((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn) < cus) least += 0.5f * t.per_k * k;
+  least += 3.0f;
+  int row = 0;
+  float rows_least = 0.f;
+  for (int i = 0; i < 6; ++i) {
+    const int bm = 16 * kRowShapes[i].mt, bn = 16 * kRowShapes[i].ntw;
+    const float us = 3.f + times(bm, bn) * (kRowShapes[i].fixed + 0.02f * static_cast<float>(bm + bn) * k);
+    if (i == 0 || us < rows_least) {
+      row = i;
+      rows_least = us;
+    }
+  }
+  return rows_least < least ? -1 - row : best;
 }
 
-// Rows that tiles take: 16-byte aligned, readable to a whole 16 columns, and, as rows are addressed
+// Rows for direct-to-LDS loads: 16-byte aligned, readable to a whole 16 columns, and, as rows are addressed
 // by 32-bit offsets, at most 2^23 bytes apart.
-static bool tiles_fit(const LinearArgs& a, bool padded) {
+static bool rows_fit(const LinearArgs& a, bool padded) {
   const int64_t at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w)) | a.xs | a.ws;
   return at % 16 == 0 && (padded || a.K % 16 == 0) && a.xs <= 1 << 23 && a.ws <= 1 << 23;
 }
 
 template <typename T>
 static int launch_linear(const LinearArgs& a, bool padded, hipStream_t st) {
-  if (a.M <= 16) return launch_rows8<T, 8, 1, 1>(a, st);
-  if (a.M <= 32) return launch_rows8<T, 8, 1, 2>(a, st);
-  if (a.M <= kRowsMax) return launch_rows8<T, 8, 1, 4>(a, st);
-  if (!tiles_fit(a, padded)) return TS_EUNSUPPORTED;
-  switch (pick_shape(a.M, a.N, a.K)) {
+  const bool aligned = rows_fit(a, padded);
+  const int kernel = pick_kernel(a.M, a.N, a.K);
+  if (kernel >= 0 && !aligned) return TS_EUNSUPPORTED;
+  switch (kernel) {
+    case -1: return launch_rows8<T, 1, 1>(a, aligned, st);
+    case -2: return launch_rows8<T, 2, 1>(a, aligned, st);
+    case -3: return launch_rows8<T, 2, 2>(a, aligned, st);
+    case -4: return launch_rows8<T, 4, 1>(a, aligned, st);
+    case -5: return launch_rows8<T, 4, 2>(a, aligned, st);
+    case -6: return launch_rows8<T, 4, 4>(a, aligned, st);
     case 0: return launch_tiles<T, 4, 2, 2, 4, 128, 2>(a, st);
     case 1: return launch_tiles<T, 3, 2, 2, 2, 128, 2>(a, st);
     case 2: return launch_tiles<T, 2, 1, 2, 4, 128, 3>(a, st);

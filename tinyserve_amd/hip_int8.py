@@ -31,7 +31,7 @@ from tinyserve_amd import _lib
 PLAIN, NORM, ADD_NORM, SILU = 0, 1, 2, 3
 MAX_K = 131071  # products of longer rows could pass an int32
 MAX_DIM = 1 << 30  # rows or columns of one call
-ROWS_MAX, MAX_STRIDE = 128, 1 << 23  # of ts_int8_linear: rows read as they are, and bytes between tiled ones
+MAX_STRIDE = 1 << 23  # bytes between rows that ts_int8_linear reads in tiles
 
 
 class Int8Rows(NamedTuple):
@@ -42,28 +42,35 @@ class Int8Rows(NamedTuple):
     scale: torch.Tensor
 
 
-def _call(dev: int, name: str, *args: object) -> None:
-    """Launch on ``dev``'s current stream, whichever device is current."""
+def _call(dev: int, name: str, *args: object) -> int:
+    """Launch on ``dev``'s current stream, whichever device is current; the status."""
     if torch._C._cuda_getDevice() == dev:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        return _lib.call_status(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return _lib.call_status(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _aligned(q: torch.Tensor) -> bool:
-    """Whether rows start at multiples of 16 bytes and may be read to a whole 16 columns."""
+def _readable(q: torch.Tensor) -> bool:
+    """Whether every row may be read up to a whole 16 columns."""
     m, k = q.shape
-    return (q.data_ptr() % 16 == 0 and q.stride(0) % 16 == 0 and
-            (k % 16 == 0 or q.storage_offset() + (m - 1) * q.stride(0) + (k + 15) // 16 * 16 <= q.untyped_storage().nbytes()))  # fmt: skip
+    need = (k + 15) // 16 * 16
+    return q.stride(0) >= need and q.storage_offset() + (m - 1) * q.stride(0) + need <= q.untyped_storage().nbytes()
 
 
 def _padded(q: torch.Tensor, dev: int) -> torch.Tensor:
-    """A copy of ``q`` whose rows are 16-byte aligned and padded with zeros."""
+    """``q``, or where its rows are not 16-byte aligned, readable to a whole 16 columns and at
+    most ``MAX_STRIDE`` apart, a copy of it with rows that are, padded with zeros."""
     m, k = q.shape
+    if q.data_ptr() % 16 == 0 and q.stride(0) % 16 == 0 and q.stride(0) <= MAX_STRIDE and (k % 16 == 0 or _readable(q)):
+        return q
     out = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=q.device)
-    _call(dev, "ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k)
+    _raise(_call(dev, "ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k), "ts_int8_pad_rows")
     return out
+
+
+def _raise(rc: int, name: str) -> None:
+    if rc:
+        raise ValueError(f"{name}: {_lib.load().ts_strerror(rc).decode()}")
 
 
 def _check_matrix(x: torch.Tensor, what: str) -> None:
@@ -102,9 +109,10 @@ def _quantize(form: int, x: torch.Tensor, y: torch.Tensor | None, weight: torch.
     q = torch.empty((t, (n + 15) // 16 * 16), dtype=torch.int8, device=x.device)
     scale = torch.empty(t, dtype=torch.float32, device=x.device)
     if t and n:
-        _call(dev, "ts_int8_quantize_rows", x.data_ptr(), None if y is None else y.data_ptr(),
-              None if weight is None else weight.data_ptr(), q.data_ptr(), scale.data_ptr(), t, n, x.stride(0),
-              0 if y is None else y.stride(0), q.stride(0), eps, form, _lib.DTYPES[x.dtype])  # fmt: skip
+        _raise(_call(dev, "ts_int8_quantize_rows", x.data_ptr(), None if y is None else y.data_ptr(),
+                     None if weight is None else weight.data_ptr(), q.data_ptr(), scale.data_ptr(), t, n, x.stride(0),
+                     0 if y is None else y.stride(0), q.stride(0), eps, form, _lib.DTYPES[x.dtype]),
+               "ts_int8_quantize_rows")  # fmt: skip
     elif t:
         scale.zero_()  # rows of no columns
     return Int8Rows(q if q.shape[1] == n else q[:, :n], scale)
@@ -158,8 +166,8 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
 
     Args:
         x: ``[M, K]`` tokens. w: ``[N, K]`` weights, a scale per output channel. K up to 131071;
-            over 128 tokens, rows that do not start at multiples of 16 bytes (the functions
-            here make them so) are copied first.
+            rows that do not start at multiples of 16 bytes (the functions here make them so)
+            are copied first where the product runs in tiles.
         out: ``[M, N]`` in ``dtype``, unit column stride (default: a new tensor).
     """
     xq, xs = x
@@ -184,13 +192,14 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
         if _lib.require_device(out) != dev:
             raise ValueError("out is on another device")
     if m and n:
-        if m > ROWS_MAX:  # read in tiles: rows that are not 16-byte aligned are copied first
-            if not _aligned(xq) or xq.stride(0) > MAX_STRIDE:
-                xq = _padded(xq, dev)
-            if not _aligned(wq) or wq.stride(0) > MAX_STRIDE:
-                wq = _padded(wq, dev)
-        _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-              ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, int(m > ROWS_MAX), code)  # fmt: skip
+        padded = k % 16 == 0 or (_readable(xq) and _readable(wq))
+        rc = _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+                   ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, padded, code)  # fmt: skip
+        if rc == _lib.TS_EUNSUPPORTED:  # read in tiles, which need aligned rows
+            xq, wq = _padded(xq, dev), _padded(wq, dev)
+            rc = _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+                       ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, 1, code)  # fmt: skip
+        _raise(rc, "ts_int8_linear")
     return out
 
 
@@ -224,6 +233,6 @@ def _rows_of(table: Int8Rows, ids: torch.Tensor | None, dtype: torch.dtype) -> t
     out = torch.empty((t, n), dtype=dtype, device=q.device)
     if t and n:
         at = None if ids is None else ids.to(torch.int64).contiguous()
-        _call(dev, "ts_int8_embedding", q.data_ptr(), q.stride(0), scale.data_ptr(), v, _lib.ptr(at), out.data_ptr(),
-              out.stride(0), t, n, code)  # fmt: skip
+        _raise(_call(dev, "ts_int8_embedding", q.data_ptr(), q.stride(0), scale.data_ptr(), v, _lib.ptr(at),
+                     out.data_ptr(), out.stride(0), t, n, code), "ts_int8_embedding")  # fmt: skip
     return out
