@@ -42,12 +42,10 @@ class Int8Rows(NamedTuple):
     scale: torch.Tensor
 
 
-def _call(dev: int, name: str, *args: object) -> int:
-    """Launch on ``dev``'s current stream, whichever device is current; the status."""
-    if torch._C._cuda_getDevice() == dev:
-        return _lib.call_status(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    with torch.cuda.device(dev):
-        return _lib.call_status(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+_current_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+_empty = torch.empty
+_INT8, _FLOAT = torch.int8, torch.float32
 
 
 def _readable(q: torch.Tensor) -> bool:
@@ -63,101 +61,100 @@ def _padded(q: torch.Tensor, dev: int) -> torch.Tensor:
     m, k = q.shape
     if q.data_ptr() % 16 == 0 and q.stride(0) % 16 == 0 and q.stride(0) <= MAX_STRIDE and (k % 16 == 0 or _readable(q)):
         return q
-    out = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=q.device)
-    _raise(_call(dev, "ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k), "ts_int8_pad_rows")
+    out = _empty((m, (k + 15) // 16 * 16), dtype=_INT8, device=q.device)
+    _lib.call("ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k, _stream(dev))
     return out
 
 
-def _raise(rc: int, name: str) -> None:
-    if rc:
-        raise ValueError(f"{name}: {_lib.load().ts_strerror(rc).decode()}")
-
-
-def _check_matrix(x: torch.Tensor, what: str) -> None:
-    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError(f"{what} must be a row-contiguous [T, N] tensor, got {tuple(x.shape)}")
-    if x.dtype not in _lib.DTYPES:
+def _matrix(x: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """Rows, columns and dtype code of a float matrix ``[T, N]``."""
+    code = _lib.DTYPES.get(x.dtype)
+    if code is None:
         raise ValueError(f"unsupported dtype {x.dtype}: float32, float16 or bfloat16")
-    _check_dims(x, what)
+    if x.dim() != 2:
+        raise ValueError(f"{what} must be a [T, N] tensor, got {tuple(x.shape)}")
+    t, n = x.shape
+    if x.stride(1) != 1 and n > 1:
+        raise ValueError(f"{what} must be row-contiguous, got {tuple(x.shape)} with strides {x.stride()}")
+    if t > MAX_DIM or n > MAX_DIM:
+        raise ValueError(f"{what}: at most {MAX_DIM} rows and columns, got {(t, n)}")
+    return t, n, code
 
 
-def _check_dims(x: torch.Tensor, what: str) -> None:
-    if x.shape[0] > MAX_DIM or x.shape[1] > MAX_DIM:
-        raise ValueError(f"{what}: at most {MAX_DIM} rows and columns, got {tuple(x.shape)}")
+def _norm_args(weight: torch.Tensor, x: torch.Tensor, n: int, eps: float) -> None:
+    if weight.dtype is not x.dtype or weight.shape != (n,) or not weight.is_contiguous():
+        raise ValueError(f"the weight must be a contiguous {x.dtype} vector of {n}, got {weight.dtype} {tuple(weight.shape)}")
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps}")
 
 
-def _check_weight(weight: torch.Tensor, x: torch.Tensor) -> None:
-    if weight.shape != (x.shape[1],) or weight.dtype != x.dtype or not weight.is_contiguous():
-        raise ValueError(f"the weight must be a contiguous {x.dtype} vector of {x.shape[1]}, "
-                         f"got {weight.dtype} {tuple(weight.shape)}")  # fmt: skip
-
-
-def _check_rows(r: Int8Rows, what: str) -> None:
+def _codes(r: Int8Rows, what: str) -> tuple[int, int]:
+    """Rows and columns of an ``Int8Rows``."""
     q, scale = r
-    if q.dtype != torch.int8 or q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1):
-        raise ValueError(f"{what}: codes must be row-contiguous int8 [M, K], got {q.dtype} {tuple(q.shape)}")
-    _check_dims(q, what)
-    if scale.dtype != torch.float32 or scale.shape != (q.shape[0],) or not scale.is_contiguous():
-        raise ValueError(f"{what}: scales must be contiguous float32 [{q.shape[0]}], got {scale.dtype} {tuple(scale.shape)}")
+    if q.dtype is not _INT8 or q.dim() != 2:
+        raise ValueError(f"{what}: codes must be int8 [M, K], got {q.dtype} {tuple(q.shape)}")
+    m, k = q.shape
+    if q.stride(1) != 1 and k > 1:
+        raise ValueError(f"{what}: codes must be row-contiguous, got {(m, k)} with strides {q.stride()}")
+    if scale.dtype is not _FLOAT or scale.shape != (m,) or not scale.is_contiguous():
+        raise ValueError(f"{what}: scales must be contiguous float32 [{m}], got {scale.dtype} {tuple(scale.shape)}")
+    if m > MAX_DIM or k > MAX_DIM:
+        raise ValueError(f"{what}: at most {MAX_DIM} rows and columns, got {(m, k)}")
+    return m, k
 
 
-def _quantize(form: int, x: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor | None, eps: float,
-              n: int) -> Int8Rows:  # fmt: skip
+def _quantize(form: int, x: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor | None, eps: float, dev: int,
+              t: int, n: int, code: int) -> Int8Rows:  # fmt: skip
     """One launch of ``ts_int8_quantize_rows``. Codes' rows start at multiples of 16 bytes."""
-    t = x.shape[0]
-    dev = _lib.require_device(x, *(z for z in (y, weight) if z is not None))
-    q = torch.empty((t, (n + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    scale = torch.empty(t, dtype=torch.float32, device=x.device)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return _quantize(form, x, y, weight, eps, dev, t, n, code)
+    stride = (n + 15) & ~15
+    q = _empty((t, stride), dtype=_INT8, device=x.device)
+    scale = _empty(t, dtype=_FLOAT, device=x.device)
     if t and n:
-        _raise(_call(dev, "ts_int8_quantize_rows", x.data_ptr(), None if y is None else y.data_ptr(),
-                     None if weight is None else weight.data_ptr(), q.data_ptr(), scale.data_ptr(), t, n, x.stride(0),
-                     0 if y is None else y.stride(0), q.stride(0), eps, form, _lib.DTYPES[x.dtype]),
-               "ts_int8_quantize_rows")  # fmt: skip
+        _lib.call("ts_int8_quantize_rows", x.data_ptr(), y if y is None else y.data_ptr(),
+                  weight if weight is None else weight.data_ptr(), q.data_ptr(), scale.data_ptr(), t, n, x.stride(0),
+                  0 if y is None else y.stride(0), stride, eps, form, code, _stream(dev))  # fmt: skip
     elif t:
         scale.zero_()  # rows of no columns
-    return Int8Rows(q if q.shape[1] == n else q[:, :n], scale)
+    return Int8Rows(q if stride == n else q[:, :n], scale)
 
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """Rows of ``x [T, N]`` in 8 bits: ``a = max|x[t]|``, ``q = rint(x * (127 / a))``,
     ``scale = a / 127``. A row of zeros (or below 2^-100) gets scale 0, one that holds a NaN or
     an infinity scale NaN; both get zero codes."""
-    _check_matrix(x, "x")
-    return _quantize(PLAIN, x, None, None, 0.0, x.shape[1])
+    t, n, code = _matrix(x, "x")
+    return _quantize(PLAIN, x, None, None, 0.0, _lib.require_device(x), t, n, code)
 
 
 def rms_norm_rows_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> Int8Rows:
     """``quantize_rows`` of RMSNorm of each row of ``x``, in one launch. The norm is not rounded
     to x's dtype before it is quantised (``rms_norm_rows`` rounds twice). ``eps`` is positive."""
-    _check_matrix(x, "x")
-    _check_weight(weight, x)
-    return _quantize(NORM, x, None, weight, _eps(eps), x.shape[1])
+    t, n, code = _matrix(x, "x")
+    _norm_args(weight, x, n, eps)
+    return _quantize(NORM, x, None, weight, eps, _lib.require_device(x, weight), t, n, code)
 
 
 def add_rms_norm_rows_int8(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: float) -> Int8Rows:
     """``x.add_(y)``, rounded to its dtype, then ``rms_norm_rows_int8(x, weight, eps)``, in one
     launch. ``x`` is updated in place; its rows must not overlap each other's, nor ``y``'s unless
     ``y`` is ``x``."""
-    _check_matrix(x, "x")
-    _check_weight(weight, x)
-    if y.shape != x.shape or y.dtype != x.dtype or (y.stride(1) != 1 and y.shape[1] > 1):
+    t, n, code = _matrix(x, "x")
+    _norm_args(weight, x, n, eps)
+    if y.dtype is not x.dtype or y.shape != x.shape or (y.stride(1) != 1 and n > 1):
         raise ValueError(f"y must be row-contiguous {tuple(x.shape)} {x.dtype}, got {tuple(y.shape)} {y.dtype}")
-    return _quantize(ADD_NORM, x, y, weight, _eps(eps), x.shape[1])
-
-
-def _eps(eps: float) -> float:
-    if not eps > 0:
-        raise ValueError(f"eps must be positive, got {eps}")
-    return float(eps)
+    return _quantize(ADD_NORM, x, y, weight, eps, _lib.require_device(x, y, weight), t, n, code)
 
 
 def silu_mul_int8(gate_up: torch.Tensor) -> Int8Rows:
     """``quantize_rows(F.silu(gate) * up)`` of ``[gate | up]`` rows ``[T, 2N]``, in one launch,
     in float32 up to the 8 bits (``silu_mul`` rounds each factor to the dtype)."""
-    _check_matrix(gate_up, "gate_up")
-    if gate_up.shape[1] % 2:
-        raise ValueError(f"need [gate | up] rows of an even width, got {tuple(gate_up.shape)}")
-    return _quantize(SILU, gate_up, None, None, 0.0, gate_up.shape[1] // 2)
+    t, n, code = _matrix(gate_up, "gate_up")
+    if n % 2:
+        raise ValueError(f"need [gate | up] rows of an even width, got {(t, n)}")
+    return _quantize(SILU, gate_up, None, None, 0.0, _lib.require_device(gate_up), t, n // 2, code)
 
 
 def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -170,36 +167,40 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
             are copied first where the product runs in tiles.
         out: ``[M, N]`` in ``dtype``, unit column stride (default: a new tensor).
     """
+    m, k = _codes(x, "x")
+    n, kw = _codes(w, "w")
     xq, xs = x
     wq, ws = w
-    _check_rows(x, "x")
-    _check_rows(w, "w")
-    m, k = xq.shape
-    n = wq.shape[0]
-    if wq.shape[1] != k:
-        raise ValueError(f"x has {k} columns but w is {tuple(wq.shape)}")
+    if kw != k:
+        raise ValueError(f"x has {k} columns but w is {(n, kw)}")
     if k > MAX_K:
         raise ValueError(f"K is at most {MAX_K} (the sums are int32), got {k}")
     code = _lib.DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
     dev = _lib.require_device(xq, xs, wq, ws)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return int8_linear(x, w, dtype, out)
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=xq.device)
+        out = _empty((m, n), dtype=dtype, device=xq.device)
+        stride = n
     else:
         if out.shape != (m, n) or out.dtype != dtype or (out.stride(1) != 1 and n > 1) or (m > 1 and out.stride(0) < n):
             raise ValueError(f"out must be {dtype} [{m}, {n}] with unit column stride, got {out.dtype} {tuple(out.shape)}")
         if _lib.require_device(out) != dev:
             raise ValueError("out is on another device")
+        stride = out.stride(0)
     if m and n:
         padded = k % 16 == 0 or (_readable(xq) and _readable(wq))
-        rc = _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-                   ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, padded, code)  # fmt: skip
-        if rc == _lib.TS_EUNSUPPORTED:  # read in tiles, which need aligned rows
+        rc = _lib.call_status("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+                              ws.data_ptr(), out.data_ptr(), stride, m, n, k, padded, code, _stream(dev))  # fmt: skip
+        if rc == _lib.TS_EUNSUPPORTED:  # it runs in tiles, which need aligned rows
             xq, wq = _padded(xq, dev), _padded(wq, dev)
-            rc = _call(dev, "ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-                       ws.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, 1, code)  # fmt: skip
-        _raise(rc, "ts_int8_linear")
+            _lib.call("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+                      ws.data_ptr(), out.data_ptr(), stride, m, n, k, 1, code, _stream(dev))  # fmt: skip
+        elif rc:
+            raise ValueError(f"ts_int8_linear: {_lib.load().ts_strerror(rc).decode()}")
     return out
 
 
@@ -218,21 +219,28 @@ def dequantize_rows(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
 
 
 def _rows_of(table: Int8Rows, ids: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
+    v, n = _codes(table, "table")
     q, scale = table
-    _check_rows(table, "table")
     code = _lib.DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
-    v, n = q.shape
-    t = v if ids is None else ids.shape[0]
-    if t and not v:
-        raise ValueError("the table has no rows")
-    if t > MAX_DIM:
-        raise ValueError(f"at most {MAX_DIM} ids, got {t}")
-    dev = _lib.require_device(q, scale) if ids is None else _lib.require_device(q, scale, ids)
-    out = torch.empty((t, n), dtype=dtype, device=q.device)
+    t = v
+    if ids is None:
+        dev = _lib.require_device(q, scale)
+    else:
+        t = ids.shape[0]
+        if t and not v:
+            raise ValueError("the table has no rows")
+        if t > MAX_DIM:
+            raise ValueError(f"at most {MAX_DIM} ids, got {t}")
+        dev = _lib.require_device(q, scale, ids)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return _rows_of(table, ids, dtype)
+    out = _empty((t, n), dtype=dtype, device=q.device)
     if t and n:
-        at = None if ids is None else ids.to(torch.int64).contiguous()
-        _raise(_call(dev, "ts_int8_embedding", q.data_ptr(), q.stride(0), scale.data_ptr(), v, _lib.ptr(at),
-                     out.data_ptr(), out.stride(0), t, n, code), "ts_int8_embedding")  # fmt: skip
+        if ids is not None and (ids.dtype is not torch.int64 or not ids.is_contiguous()):
+            ids = ids.to(torch.int64).contiguous()
+        _lib.call("ts_int8_embedding", q.data_ptr(), q.stride(0), scale.data_ptr(), v,
+                  ids if ids is None else ids.data_ptr(), out.data_ptr(), n, t, n, code, _stream(dev))  # fmt: skip
     return out
