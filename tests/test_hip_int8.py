@@ -272,6 +272,24 @@ def test_rows_that_have_no_scale(form: str, n: int, dtype: torch.dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [5, 40, 700, 40000])
+def test_gates_of_every_size(n: int, dtype: torch.dtype) -> None:
+    """SiLU where its exponential overflows, underflows or does neither, one size a row."""
+    gates = [0.0, 1e-6, -1e-6, 1.0, -1.0, 10.0, -10.0, 50.0, -50.0, 80.0, -80.0, 88.0, 89.0, 130.0, 1e4, 6e4]
+    x = torch.randn(len(gates), 2 * n, generator=torch.Generator().manual_seed(n)).to(dtype)
+    x[:, :n] = torch.tensor(gates)[:, None].to(dtype)
+    check_rows("silu", silu_mul_int8(x.to(DEVICE)), {"x": x})
+    # Where exp(-g) passes float32 the value is 0 to within 1e-36: the rest of the row decides.
+    x[:, 0] = torch.tensor([-88.5, -89.0, -95.0, -130.0, -1e3, -6e4] * 3)[: len(gates)].to(dtype)
+    check_rows("silu", silu_mul_int8(x[3:].to(DEVICE)), {"x": x[3:]})
+    if dtype == torch.float32:
+        x[:, :n], x[:, n:] = torch.tensor([3e38, -3e38] * 8)[:, None], 0.1
+        got = silu_mul_int8(x.to(DEVICE))
+        assert bool((got.q[::2] == 127).all()) and bool((got.scale[1::2] < 1e-36).all())
+
+
+@pytest.mark.gpu
 def test_sums_of_squares_past_float32_are_nan_rows() -> None:
     x = torch.full((2, 64), 2.0**64)
     x[1] = 2.0**50

@@ -51,7 +51,21 @@ __device__ __forceinline__ Pack16<T> load_chunk(const T* row, int i, int N) {
   return r;
 }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+// g / (1 + exp(-g)), within about 2^-21: exp(-g) as 2^t of t = -g log2(e), with the rounding of t put
+// right to first order (t alone would be off by |g| 2^-24), and the quotient by the reciprocal.
+// The exponent is taken from g cut to where 2^t is finite: below -88.7 the result, under 1e-36 in
+// magnitude, is -88.7's; the last term makes an infinity or a NaN in g a NaN.
+// The hardware's exp2 and reciprocal are within one unit in the last place; expf and a correctly
+// rounded quotient made the kernel wait for its arithmetic (8192 x 8192 bf16 82 us, now 68).
+__device__ __forceinline__ float silu(float g) {
+  constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - (float)log2(e)
+  constexpr float kLn2 = 0.693147180559945f;
+  const float cut = fminf(fmaxf(g, -88.7f), 88.7f);
+  const float t = -cut * kLog2e;
+  const float off = fmaf(-cut, kLog2e, -t) - cut * kLog2eLow;
+  const float e = fast_exp2(t);
+  return fmaf(g, 0.0f, fmaxf(g, -88.7f) * __builtin_amdgcn_rcpf(1.0f + fmaf(e, off * kLn2, e)));
+}
 
 // |v| as bits: ordered as the magnitudes are, infinities above every finite value and NaN above
 // those, so one unsigned maximum carries all three.
@@ -62,13 +76,16 @@ __device__ __forceinline__ uint32_t xor_lane_u(uint32_t x) {
   return __float_as_uint(xor_lane<OFF>(__uint_as_float(x)));
 }
 
-__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+// The largest x of each group of N consecutive lanes.
+template <int N>
+__device__ __forceinline__ uint32_t group_umax(uint32_t x) {
   x = max(x, xor_lane_u<1>(x));
   x = max(x, xor_lane_u<2>(x));
   x = max(x, xor_lane_u<4>(x));
   x = max(x, xor_lane_u<8>(x));
-  x = max(x, xor_lane_u<16>(x));
-  return max(x, xor_lane_u<32>(x));
+  if constexpr (N >= 32) x = max(x, xor_lane_u<16>(x));
+  if constexpr (N >= 64) x = max(x, xor_lane_u<32>(x));
+  return x;
 }
 
 // A row's factor for its codes (0: all codes are zero) and its scale, from the largest
@@ -96,9 +113,16 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top, float ss, int N, flo
   return r;
 }
 
-// The code of v, in the low byte. A NaN row has inv 0, and 0 * inf or NaN is masked by it.
-__device__ __forceinline__ uint32_t code(float v, float inv) {
-  return static_cast<uint32_t>(static_cast<int>(rintf(inv == 0.0f ? 0.0f : v * inv))) & 0xffu;
+// The codes of four values, a byte each. Adding 1.5 * 2^23 leaves rint(v * inv), at most 127, in
+// the sum's low bits. A row without a scale has inv 0, whatever its values: all codes zero.
+__device__ __forceinline__ uint32_t codes4(const float* v, float inv) {
+  constexpr float kMagic = 12582912.0f;
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fmaf(v[e], inv, kMagic));
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);  // low bytes of b[0], b[1]
+  const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);  // of b[2], b[3], above them
+  return inv == 0.0f ? 0u : lo | hi;
 }
 
 struct QuantArgs {
@@ -113,15 +137,16 @@ struct QuantArgs {
   float eps;
 };
 
-// WAVES waves per row (WAVES == 1: the workgroup's waves take a row each), CPT chunks of E
-// elements per lane.
-template <typename T, int FORM, int WAVES, int CPT>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void quantize_rows_kernel(const QuantArgs a) {
+// TPR threads per row, CPT chunks of E elements each; up to 64 threads a workgroup takes 256 / TPR
+// rows, else one.
+template <typename T, int FORM, int TPR, int CPT>
+__global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel(const QuantArgs a) {
   constexpr int E = Pack16<T>::N;
-  constexpr int TPR = WAVES * kWave;
+  constexpr int LPR = TPR < kWave ? TPR : kWave;  // lanes of a wave on one row
+  constexpr int WAVES = TPR / LPR;
   const int wave = threadIdx.x / kWave;
-  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWave) + wave : blockIdx.x;
-  const int t = WAVES == 1 ? threadIdx.x % kWave : threadIdx.x;
+  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR : blockIdx.x;
+  const int t = threadIdx.x % TPR;
   if (WAVES == 1 && row >= a.rows) return;
   const int N = a.N;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
@@ -169,8 +194,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void quantize_row
     }
   }
 
-  top = wave_umax(top);
-  if constexpr (FORM == kNorm || FORM == kAddNorm) ss = group_sum<kWave>(ss);
+  top = group_umax<LPR>(top);
+  if constexpr (FORM == kNorm || FORM == kAddNorm) ss = group_sum<LPR>(ss);
   if constexpr (WAVES > 1) {
     __shared__ uint32_t tops[WAVES];
     __shared__ float sums[WAVES];
@@ -197,9 +222,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void quantize_row
     if (i >= N) continue;
     uint32_t word[E / 4];
 #pragma unroll
-    for (int k = 0; k < E / 4; ++k)
-      word[k] = code(v[c][4 * k], r.inv) | code(v[c][4 * k + 1], r.inv) << 8 | code(v[c][4 * k + 2], r.inv) << 16 |
-                code(v[c][4 * k + 3], r.inv) << 24;
+    for (int k = 0; k < E / 4; ++k) word[k] = codes4(&v[c][4 * k], r.inv);
     // Whole words: the row's padding, up to its stride, takes zeros.
     if constexpr (E == 8) *reinterpret_cast<uint2*>(q + i) = uint2{word[0], word[1]};
     else *reinterpret_cast<uint32_t*>(q + i) = word[0];
@@ -236,7 +259,7 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
     if constexpr (FORM == kNorm || FORM == kAddNorm) ss = fmaf(f, f, ss);
     top = max(top, magnitude(value(i, f)));
   }
-  top = wave_umax(top);
+  top = group_umax<kWave>(top);
   ss = group_sum<kWave>(ss);
   __shared__ uint32_t tops[16];
   __shared__ float sums[16];
@@ -258,7 +281,8 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
     float f;
     if constexpr (FORM == kAddNorm) f = to_f32(xo[i]);
     else f = to_f32(x[i]);
-    q[i] = static_cast<int8_t>(code(value(i, f), r.inv));
+    const float v[4] = {value(i, f), 0.f, 0.f, 0.f};
+    q[i] = static_cast<int8_t>(codes4(v, r.inv) & 0xffu);
   }
 }
 
@@ -266,20 +290,26 @@ template <typename T, int FORM>
 static int launch_quantize(const QuantArgs& a, hipStream_t st) {
   constexpr int E = Pack16<T>::N;
   const int chunks = (a.N + E - 1) / E;
+  // Few rows: more threads on each, one or two chunks a thread.
   const bool few = a.rows < 2 * compute_units();
-#define TS_QUANT(W, C)                                                                                     \
-  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, W, C>), dim3((W) == 1 ? (a.rows + 3) / 4 : a.rows),    \
-                     dim3((W) == 1 ? 256 : (W) * kWave), 0, st, a)
+#define TS_QUANT(P, C)                                                                                       \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, P, C>),                                                  \
+                     dim3((P) <= kWave ? (a.rows + 256 / (P) - 1) / (256 / (P)) : a.rows), dim3((P) <= kWave ? 256 : (P)), 0, st, a)
   if (a.N < E || chunks > 4096) hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(1024), 0, st, a);
-  else if (chunks <= 64) TS_QUANT(1, 1);
-  else if (few && chunks <= 256) TS_QUANT(4, 1);
-  else if (few && chunks <= 512) TS_QUANT(4, 2);
-  else if (chunks <= 128) TS_QUANT(1, 2);
-  else if (chunks <= 256) TS_QUANT(1, 4);
-  else if (chunks <= 512) TS_QUANT(4, 2);
-  else if (chunks <= 1024) TS_QUANT(4, 4);
-  else if (chunks <= 2048) TS_QUANT(16, 2);
-  else TS_QUANT(16, 4);
+  else if (chunks <= 16) TS_QUANT(16, 1);
+  else if (chunks <= 32) TS_QUANT(32, 1);
+  else if (chunks <= 64) TS_QUANT(64, 1);
+  else if (few && chunks <= 256) TS_QUANT(256, 1);
+  else if (few && chunks <= 512) TS_QUANT(256, 2);
+  else if (chunks <= 128) TS_QUANT(64, 2);
+  else if (chunks <= 256) TS_QUANT(64, 4);
+  else if (chunks <= 512) TS_QUANT(256, 2);
+  else if (chunks <= 768) TS_QUANT(256, 3);
+  else if (chunks <= 1024) TS_QUANT(256, 4);
+  else if (chunks <= 1536) TS_QUANT(512, 3);
+  else if (chunks <= 2048) TS_QUANT(512, 4);
+  else if (chunks <= 3072) TS_QUANT(1024, 3);
+  else TS_QUANT(1024, 4);
 #undef TS_QUANT
   return launch_status();
 }
