@@ -24,6 +24,14 @@ projections through library GEMMs instead:
     h = add_rms_norm_rows(x, attn @ W_o^T)          (rounded, then added in place)
     down = silu_mul(h @ W_gate_up^T) @ W_down^T     (added by the next norm)
 
+With 8-bit weights (``int8_weights``: every matrix ``quantize_rows``, the table of embeddings
+and output head once for both) every product of the step, the head's too, is ``int8_linear``,
+for any number of rows and any dtype of the activations (hip_int8.py):
+
+    h = add_rms_norm_rows_int8(x, previous layer's down product); qkv = int8_linear(h, W_qkv); ...
+    h = add_rms_norm_rows_int8(x, int8_linear(quantize_rows(attn), W_o))
+    down = int8_linear(silu_mul_int8(int8_linear(h, W_gate_up)), W_down)
+
 Weights are random (no checkpoints here): linear weights ~ N(0, 0.02) in the model dtype,
 norm weights 1 + 0.1 N(0, 1). The KV pool has the reference's layout (kv_cache.py:20-50):
 per layer ``[num_blocks * block_size + block_size, Hkv, D]``, the last block being the
@@ -40,7 +48,8 @@ import torch.nn.functional as F
 
 from collections.abc import Callable
 
-from tinyserve_amd import hip_attention, hip_fused, hip_prefill, hip_rows
+from tinyserve_amd import hip_attention, hip_fused, hip_int8, hip_prefill, hip_rows
+from tinyserve_amd.hip_int8 import Int8Rows
 from tinyserve_amd.step_inputs import Batch, DecodeInputs, host_ints
 
 HEAD_MIN_ROWS = 8  # the output head runs on at least this many rows (model.py:64)
@@ -98,6 +107,12 @@ def random_weights(shape: ModelShape, dtype: torch.dtype = torch.float16,
     return w
 
 
+def int8_weights(weights: dict[str, torch.Tensor]) -> dict[str, torch.Tensor | Int8Rows]:
+    """``weights`` (on a HIP device) with every matrix in 8 bits, a scale per output channel
+    (``hip_int8.quantize_rows``); the norms' vectors as they are. For ``DecodeStep``."""
+    return {name: hip_int8.quantize_rows(w) if w.dim() == 2 else w for name, w in weights.items()}
+
+
 class KVPool:
     """The KV cache tensors (kv_cache.py:20-50): ``k``, ``v`` of shape
     ``[L, num_blocks * block_size + block_size, Hkv, D]``; block ``num_blocks`` is the
@@ -132,25 +147,32 @@ class DecodeStep:
 
     ``num_splits``: the decode kernel's split count (None: the launcher's policy; the
     reference's config-5 step forces 16). ``projections``: "rows" (the row-batch HIP
-    kernels), "library" (library GEMMs) or "auto" (rows where the dtype and shapes allow,
-    for steps of up to ``ROWS_MAX`` rows)."""
+    kernels), "library" (library GEMMs), "int8" (8-bit weights, ``int8_weights``) or "auto"
+    (int8 where the weights are; else rows where the dtype and shapes allow, for steps of up
+    to ``ROWS_MAX`` rows)."""
 
-    def __init__(self, shape: ModelShape, weights: dict[str, torch.Tensor], pool: KVPool,
+    def __init__(self, shape: ModelShape, weights: dict[str, torch.Tensor | Int8Rows], pool: KVPool,
                  num_splits: int | None = None, projections: str = "auto") -> None:  # fmt: skip
         self.shape = shape
         self.w = weights
         self.pool = pool
         self.num_splits = num_splits
         self.scale = shape.head_dim**-0.5
-        dtype = weights["model.embed_tokens.weight"].dtype
+        dtype = weights["model.norm.weight"].dtype
+        int8 = isinstance(weights["model.embed_tokens.weight"], Int8Rows)
         fits = (hip_rows.supported(dtype) and shape.hidden % 32 == 0 and shape.intermediate % 32 == 0
                 and shape.q_size % 32 == 0 and shape.hidden <= 4096)  # fmt: skip
-        if projections not in ("auto", "rows", "library"):
-            raise ValueError(f"projections must be 'auto', 'rows' or 'library', got {projections!r}")
+        if projections not in ("auto", "rows", "library", "int8"):
+            raise ValueError(f"projections must be 'auto', 'rows', 'library' or 'int8', got {projections!r}")
+        if projections != "auto" and int8 != (projections == "int8"):
+            raise ValueError(f"projections {projections!r} with {'8-bit' if int8 else 'float'} weights")
         if projections == "rows" and not fits:
             raise ValueError(f"the row-batch projections need fp16/bf16 and 32-aligned widths (hidden <= 4096), "
                              f"got {dtype} and {shape}")  # fmt: skip
-        self.projections = projections if projections != "auto" else ("rows" if fits else "library")
+        if projections == "auto":
+            projections = "int8" if int8 else "rows" if fits else "library"
+        self.projections = projections
+        self.dtype = dtype
 
     def _attention(self, i: int, q: torch.Tensor, inputs: DecodeInputs) -> torch.Tensor:
         return hip_attention.launch_paged_decode_split(
@@ -161,7 +183,8 @@ class DecodeStep:
               attend: Callable[[int, torch.Tensor], torch.Tensor]) -> torch.Tensor:  # fmt: skip
         """One decoder layer (model.py:137-179, the fused path): the new tokens' k/v go to
         the pool at ``slots``; ``attend(i, q)`` returns the attention output for ``q``."""
-        return x.add_(self._layer(i, x, None, cos, sin, slots, attend))
+        layer = self._layer_int8 if self.projections == "int8" else self._layer
+        return x.add_(layer(i, x, None, cos, sin, slots, attend))
 
     def _layer(self, i: int, x: torch.Tensor, pending: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
                slots: torch.Tensor, attend: Callable[[int, torch.Tensor], torch.Tensor]) -> torch.Tensor:  # fmt: skip
@@ -189,6 +212,32 @@ class DecodeStep:
                                         w[p + "post_attention_layernorm.weight"], s.rms_norm_eps)  # fmt: skip
         act = hip_fused.silu_mul(F.linear(h, w[p + "mlp.gate_up_proj.weight"]))
         return F.linear(act, w[p + "mlp.down_proj.weight"])
+
+    def _layer_int8(self, i: int, x: torch.Tensor, pending: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
+                    slots: torch.Tensor, attend: Callable[[int, torch.Tensor], torch.Tensor]) -> torch.Tensor:  # fmt: skip
+        """``_layer`` with 8-bit weights: each product takes 8-bit rows and gives the step's
+        dtype; the residual stream, q, k and v stay in it."""
+        s, w, p = self.shape, self.w, f"model.layers.{i}."
+        n = x.shape[0]
+        h = self._norm_int8(x, pending, p + "input_layernorm.weight")
+        qkv = hip_int8.int8_linear(h, w[p + "self_attn.qkv_proj.weight"], self.dtype)
+        q, k, v = torch.split(qkv, [s.q_size, s.kv_size, s.kv_size], dim=1)
+        q = hip_fused.qk_norm_rope_store(
+            q.view(n, s.num_heads, s.head_dim), k.view(n, s.num_kv_heads, s.head_dim),
+            v.view(n, s.num_kv_heads, s.head_dim), w[p + "self_attn.q_norm.weight"],
+            w[p + "self_attn.k_norm.weight"], cos, sin, slots, self.pool.k[i],
+            self.pool.v[i], s.rms_norm_eps)  # fmt: skip
+        attn = hip_int8.quantize_rows(attend(i, q).reshape(n, s.q_size))
+        o = hip_int8.int8_linear(attn, w[p + "self_attn.o_proj.weight"], self.dtype)
+        h = self._norm_int8(x, o, p + "post_attention_layernorm.weight")
+        act = hip_int8.silu_mul_int8(hip_int8.int8_linear(h, w[p + "mlp.gate_up_proj.weight"], self.dtype))
+        return hip_int8.int8_linear(act, w[p + "mlp.down_proj.weight"], self.dtype)
+
+    def _norm_int8(self, x: torch.Tensor, pending: torch.Tensor | None, name: str) -> Int8Rows:
+        """The norm ``name`` of ``x`` in 8 bits, after adding ``pending`` to ``x`` in place."""
+        if pending is None:
+            return hip_int8.rms_norm_rows_int8(x, self.w[name], self.shape.rms_norm_eps)
+        return hip_int8.add_rms_norm_rows_int8(x, pending, self.w[name], self.shape.rms_norm_eps)
 
     def _layers_rows(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, slots: torch.Tensor,
                      attend: Callable[[int, torch.Tensor], torch.Tensor]) -> torch.Tensor:  # fmt: skip
@@ -222,6 +271,15 @@ class DecodeStep:
         """Logits of every token, or of ``rows`` only (model.py:181-211)."""
         s = self.shape
         cos, sin = rope_tables(s.head_dim, s.rope_theta, positions)
+        if self.projections == "int8":
+            table = self.w["model.embed_tokens.weight"]
+            x = hip_int8.int8_embedding(table, token_ids, self.dtype)
+            pending = None
+            for i in range(s.num_layers):
+                pending = self._layer_int8(i, x, pending, cos, sin, slots, attend)
+            if rows is not None:
+                x, pending = x[rows], None if pending is None else pending[rows]
+            return hip_int8.int8_linear(self._norm_int8(x, pending, "model.norm.weight"), table, torch.float32)
         x = self.w["model.embed_tokens.weight"][token_ids]
         if self.projections == "rows" and x.shape[0] <= ROWS_MAX:
             x = self._layers_rows(x, cos, sin, slots, attend)
