@@ -108,6 +108,17 @@ def same(got: torch.Tensor, want: torch.Tensor) -> bool:
     return torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
 
 
+@pytest.fixture(params=["compiled", "python"])
+def host_path(request: pytest.FixtureRequest, monkeypatch: pytest.MonkeyPatch) -> str:
+    """Both host paths of the calls: the compiled one (bound by a first call) and Python's."""
+    quantize_rows(torch.ones(1, 16, device=DEVICE))
+    if request.param == "python":
+        monkeypatch.setattr(hip_int8, "_fast", None)
+    else:
+        assert hip_int8._fast is not None
+    return request.param
+
+
 # ---- refusals (CPU) ------------------------------------------------------------------------------
 def test_refusals_come_before_the_device() -> None:
     x = torch.zeros(2, 8, dtype=torch.float16)
@@ -528,6 +539,55 @@ def test_captured_and_replayed() -> None:
         got = out.clone()
         assert torch.equal(got, chain()), seed
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("t", "n"), [(1, 16), (3, 40), (300, 257), (700, 1024)])
+def test_both_host_paths(t: int, n: int, dtype: torch.dtype, host_path: str) -> None:
+    for form in FORMS:
+        c = rows_of(t, n, dtype, seed=t, form=form)
+        d = device(c)
+        got = call(form, d)
+        assert type(got) is Int8Rows and got.q.stride(0) % 16 == 0
+        check_rows(form, got, c)
+        if form == "add":
+            assert torch.equal(d["x"].cpu().double(), definition(form, c)[2])
+    w = Int8Rows(codes(n, n, 1).to(DEVICE), scales(n, 2).to(DEVICE))
+    assert torch.equal(int8_linear(got, w, dtype).cpu(), linear_want(got, w, dtype))
+    out = torch.full((t, n + 5), 2.0, dtype=dtype, device=DEVICE)
+    view = out[:, 2 : n + 2]
+    assert int8_linear(got, w, dtype, view) is view
+    assert torch.equal(view.cpu(), linear_want(got, w, dtype)) and bool((out[:, :2] == 2).all()) and bool((out[:, n + 2 :] == 2).all())
+    want = (got.q.cpu().float() * got.scale.cpu()[:, None]).to(dtype)
+    assert torch.equal(dequantize_rows(got, dtype).cpu(), want)
+    ids = torch.arange(t - 1, -1, -1)
+    for kind in (torch.int64, torch.int32):
+        assert torch.equal(int8_embedding(got, ids.to(kind).to(DEVICE), dtype).cpu(), want.flip(0))
+
+
+@pytest.mark.gpu
+def test_both_host_paths_refuse(host_path: str) -> None:
+    x = torch.randn(4, 32, device=DEVICE).half()
+    w = torch.ones(32, dtype=torch.float16, device=DEVICE)
+    r = quantize_rows(x)
+    for op in (lambda: quantize_rows(x.t()), lambda: quantize_rows(x.double()), lambda: quantize_rows(x[0]),
+               lambda: rms_norm_rows_int8(x, w[:31], EPS), lambda: rms_norm_rows_int8(x, w.float(), EPS),
+               lambda: rms_norm_rows_int8(x, w, 0.0), lambda: add_rms_norm_rows_int8(x, x[:2], w, EPS),
+               lambda: add_rms_norm_rows_int8(x[:, :16], x[:, 8:24], w[:16], EPS),
+               lambda: add_rms_norm_rows_int8(x[:1].expand(4, 32), x, w, EPS), lambda: silu_mul_int8(x[:, :31]),
+               lambda: int8_linear(r, quantize_rows(x[:, :16].contiguous()), torch.float16),
+               lambda: int8_linear(r, r, torch.int8), lambda: int8_linear(Int8Rows(r.q, r.scale[:3]), r, torch.float16),
+               lambda: int8_linear(r, r, torch.float16, torch.empty(4, 5, dtype=torch.float16, device=DEVICE)),
+               lambda: dequantize_rows(r, torch.float64), lambda: int8_embedding(r, torch.zeros(2, device=DEVICE), torch.float16)):  # fmt: skip
+        with pytest.raises(ValueError):
+            op()
+    for op in (lambda: rms_norm_rows_int8(x, w.cpu(), EPS), lambda: add_rms_norm_rows_int8(x, x.cpu(), w, EPS),
+               lambda: int8_linear(r, Int8Rows(r.q.cpu(), r.scale.cpu()), torch.float16),
+               lambda: int8_embedding(r, torch.zeros(2, dtype=torch.int64), torch.float16)):  # fmt: skip
+        with pytest.raises(RuntimeError, match="HIP device only"):
+            op()
+    assert torch.equal(quantize_rows(x).q, r.q)  # x as it was: nothing was launched
 
 
 @pytest.mark.gpu

@@ -81,10 +81,11 @@ def build(verbose: bool = False) -> Path:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stderr}")
-    for old in PKG.glob("_fastcall*.so"):  # built from the sources of the library that goes
+    for old in (*PKG.glob("_fastcall*.so"), *PKG.glob("_fastint8*.so")):  # built from the sources of the library that goes
         old.unlink()
     tmp.replace(out)  # atomic: a process that already mapped the old file keeps it
     _build_fastcall(verbose)
+    _build_fastint8(verbose)
     return out
 
 
@@ -102,6 +103,29 @@ def _build_fastcall(verbose: bool) -> Path | None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         print(f"fastcall.c failed; launches go through ctypes:\n{proc.stderr}", file=sys.stderr)
+        return None
+    tmp.replace(out)
+    return out
+
+
+def _build_fastint8(verbose: bool) -> Path | None:
+    """The compiled host path of ``hip_int8``, against this interpreter's torch. Without a C++
+    compiler or torch's headers there is none, and the calls go through Python."""
+    import torch
+
+    cxx = shutil.which("g++") or shutil.which("c++") or hipcc()
+    root = Path(torch.__file__).resolve().parent
+    out = PKG / f"_fastint8{sysconfig.get_config_var('EXT_SUFFIX')}"
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{sysconfig.get_paths()['include']}",
+           f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           str(CSRC / "fastint8.cpp"), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]  # fmt: skip
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        print(f"fastint8.cpp failed; hip_int8 goes through Python:\n{proc.stderr}", file=sys.stderr)
         return None
     tmp.replace(out)
     return out

@@ -39,6 +39,15 @@ __device__ __forceinline__ T from_f32(float x) {
   return static_cast<T>(x);  // round to nearest even for f16 and bf16
 }
 
+// from_f32 of a product or sum that is rounded to float32 first. Without the empty asm the compiler
+// makes the operation and the conversion to f16 one v_fma_mixlo_f16, which rounds once, in some
+// places and not in others, and the same values would come out differently by where they stand.
+template <typename T>
+__device__ __forceinline__ T round_f32(float x) {
+  asm("" : "+v"(x));
+  return from_f32<T>(x);
+}
+
 template <typename T>
 __device__ __forceinline__ Pack16<T> load16(const T* p) {
   Pack16<T> r;

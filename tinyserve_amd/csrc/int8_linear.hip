@@ -62,12 +62,12 @@ __device__ __forceinline__ void store_outputs(const LinearArgs& a, int m, int n,
   if (n + 4 <= a.N) {
     typename Vec4<T>::V y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(static_cast<float>(sum[i]) * s * a.wscale[n + i]);
+    for (int i = 0; i < 4; ++i) y[i] = round_f32<T>(static_cast<float>(sum[i]) * s * a.wscale[n + i]);
     *reinterpret_cast<typename Vec4<T>::Loose*>(o) = y;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) o[i] = from_f32<T>(static_cast<float>(sum[i]) * s * a.wscale[n + i]);
+      if (n + i < a.N) o[i] = round_f32<T>(static_cast<float>(sum[i]) * s * a.wscale[n + i]);
   }
 }
 
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
         const f32x4 sw = *reinterpret_cast<const f32x4*>(scales + wn * 32 * NW + c);
         typename Vec4<T>::V y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * sw[i]);
+        for (int i = 0; i < 4; ++i) y[i] = round_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * sw[i]);
         *reinterpret_cast<typename Vec4<T>::V*>(mine + (lane % 32) * kRow + c * sizeof(T)) = y;
       }
     __builtin_amdgcn_wave_barrier();

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel
     if constexpr (FORM == kAddNorm) {
       const int i = (c * TPR + t) * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) xv[c].v[e] = from_f32<T>(to_f32(xv[c].v[e]) + to_f32(sv[c].v[e]));
+      for (int e = 0; e < E; ++e) xv[c].v[e] = round_f32<T>(to_f32(xv[c].v[e]) + to_f32(sv[c].v[e]));
       T* xo = static_cast<T*>(a.xo) + row * a.xs + i;
       if (i + E <= N) {
         store16_loose(xo, xv[c]);
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
   for (int i = threadIdx.x; i < N; i += 1024) {
     float f;
     if constexpr (FORM == kAddNorm) {
-      const T s = from_f32<T>(to_f32(xo[i]) + to_f32(y[i]));
+      const T s = round_f32<T>(to_f32(xo[i]) + to_f32(y[i]));
       xo[i] = s;
       f = to_f32(s);
     } else {
@@ -327,20 +327,27 @@ static int launch_form(const QuantArgs& a, int form, hipStream_t st) {
 // ---- rows of an 8-bit table -----------------------------------------------------------------
 // out[t] = (T)(q[ids[t]] * scale[ids[t]]): one thread per 16 codes. Bound by HBM (and, for few
 // ids, by the chain id -> row). An id outside the table gives a row of NaN.
+struct TableArgs {
+  const int8_t* q;
+  const float* scale;
+  const int64_t* ids;  // null: row t itself
+  void* out;
+  int64_t qs, os, table;  // table: its rows
+  int rows, N, per_row;   // per_row: threads per row
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void int8_embedding_kernel(const int8_t* __restrict__ q, int64_t qs,
-                                                             const float* __restrict__ scale, int64_t table,
-                                                             const int64_t* __restrict__ ids, T* __restrict__ out,
-                                                             int64_t os, int rows, int N, int per_row) {
-  const int64_t total = static_cast<int64_t>(rows) * per_row;
+__global__ __launch_bounds__(256) void int8_embedding_kernel(const TableArgs a) {
+  const int N = a.N;
+  const int64_t total = static_cast<int64_t>(a.rows) * a.per_row;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t t = u / per_row;
-    const int i = static_cast<int>(u - t * per_row) * 16;
-    const int64_t id = ids ? ids[t] : t;
-    const bool in = id >= 0 && id < table;
-    const float s = in ? scale[id] : __uint_as_float(0x7fc00000u);
-    const int8_t* p = q + (in ? id : 0) * qs + i;
-    T* o = out + t * os + i;
+    const int64_t t = u / a.per_row;
+    const int i = static_cast<int>(u - t * a.per_row) * 16;
+    const int64_t id = a.ids ? a.ids[t] : t;
+    const bool in = id >= 0 && id < a.table;
+    const float s = in ? a.scale[id] : __uint_as_float(0x7fc00000u);
+    const int8_t* p = a.q + (in ? id : 0) * a.qs + i;
+    T* o = static_cast<T*>(a.out) + t * a.os + i;
     if (i + 16 <= N) {
       union {
         u32x4 raw;
@@ -352,11 +359,11 @@ __global__ __launch_bounds__(256) void int8_embedding_kernel(const int8_t* __res
       for (int k = 0; k < 16 / E; ++k) {
         Pack16<T> y;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y.v[e] = from_f32<T>(static_cast<float>(c.b[k * E + e]) * s);
+        for (int e = 0; e < E; ++e) y.v[e] = round_f32<T>(static_cast<float>(c.b[k * E + e]) * s);
         store16_loose(o + k * E, y);
       }
     } else {
-      for (int e = 0; e < N - i; ++e) o[e] = from_f32<T>(static_cast<float>(p[e]) * s);
+      for (int e = 0; e < N - i; ++e) o[e] = round_f32<T>(static_cast<float>(p[e]) * s);
     }
   }
 }
@@ -386,12 +393,11 @@ __global__ __launch_bounds__(256) void int8_pad_rows_kernel(const int8_t* __rest
 }
 
 template <typename T>
-static int launch_embedding(const int8_t* q, int64_t qs, const float* scale, int64_t table, const int64_t* ids, void* out,
-                            int64_t os, int rows, int N, hipStream_t st) {
-  const int per_row = (N + 15) / 16;
-  const int64_t blocks = (static_cast<int64_t>(rows) * per_row + 255) / 256;
+static int launch_embedding(TableArgs a, hipStream_t st) {
+  a.per_row = (a.N + 15) / 16;
+  const int64_t blocks = (static_cast<int64_t>(a.rows) * a.per_row + 255) / 256;
   hipLaunchKernelGGL(int8_embedding_kernel<T>, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256),
-                     0, st, q, qs, scale, table, ids, static_cast<T*>(out), os, rows, N, per_row);
+                     0, st, a);
   return launch_status();
 }
 
@@ -437,11 +443,12 @@ extern "C" int ts_int8_embedding(const int8_t* table, int64_t t_stride, const fl
   if (T == 0 || N == 0) return 0;
   // The rows of an empty table do not exist: there is nothing to read for any id.
   if (!table || !scale || !out || table_rows == 0 || (!ids && T > table_rows)) return TS_EINVAL;
+  const TableArgs a{table, scale, ids, out, t_stride, o_stride, table_rows, T, N, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case TS_F32: return launch_embedding<float>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
-    case TS_F16: return launch_embedding<f16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
-    default: return launch_embedding<bf16>(table, t_stride, scale, table_rows, ids, out, o_stride, T, N, st);
+    case TS_F32: return launch_embedding<float>(a, st);
+    case TS_F16: return launch_embedding<f16>(a, st);
+    default: return launch_embedding<bf16>(a, st);
   }
 }
 

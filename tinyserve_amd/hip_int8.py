@@ -22,6 +22,7 @@ allocates only its results, by torch's caching allocator, so a HIP graph can cap
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -46,6 +47,25 @@ _current_device = torch._C._cuda_getDevice
 _stream = torch._C._cuda_getCurrentRawStream
 _empty = torch.empty
 _INT8, _FLOAT = torch.int8, torch.float32
+
+
+# The compiled host path of the calls (csrc/fastint8.cpp), bound by the first call that goes
+# through Python; None where it is not built, and then every call does.
+_fast = None
+_bound = False
+
+
+def _bind_fast() -> None:
+    global _fast, _bound
+    _bound = True
+    try:
+        from tinyserve_amd import _fastint8
+    except ImportError:
+        return
+    lib = _lib.load()
+    names = ("ts_int8_quantize_rows", "ts_int8_embedding", "ts_int8_linear")
+    _fastint8.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), Int8Rows, _stream)
+    _fast = _fastint8
 
 
 def _readable(q: torch.Tensor) -> bool:
@@ -106,6 +126,8 @@ def _codes(r: Int8Rows, what: str) -> tuple[int, int]:
 def _quantize(form: int, x: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor | None, eps: float, dev: int,
               t: int, n: int, code: int) -> Int8Rows:  # fmt: skip
     """One launch of ``ts_int8_quantize_rows``. Codes' rows start at multiples of 16 bytes."""
+    if not _bound:
+        _bind_fast()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return _quantize(form, x, y, weight, eps, dev, t, n, code)
@@ -125,6 +147,8 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """Rows of ``x [T, N]`` in 8 bits: ``a = max|x[t]|``, ``q = rint(x * (127 / a))``,
     ``scale = a / 127``. A row of zeros (or below 2^-100) gets scale 0, one that holds a NaN or
     an infinity scale NaN; both get zero codes."""
+    if _fast is not None and (got := _fast.quantize(PLAIN, x, None, None, 0.0)) is not None:
+        return got
     t, n, code = _matrix(x, "x")
     return _quantize(PLAIN, x, None, None, 0.0, _lib.require_device(x), t, n, code)
 
@@ -132,6 +156,8 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
 def rms_norm_rows_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> Int8Rows:
     """``quantize_rows`` of RMSNorm of each row of ``x``, in one launch. The norm is not rounded
     to x's dtype before it is quantised (``rms_norm_rows`` rounds twice). ``eps`` is positive."""
+    if _fast is not None and (got := _fast.quantize(NORM, x, None, weight, eps)) is not None:
+        return got
     t, n, code = _matrix(x, "x")
     _norm_args(weight, x, n, eps)
     return _quantize(NORM, x, None, weight, eps, _lib.require_device(x, weight), t, n, code)
@@ -141,6 +167,8 @@ def add_rms_norm_rows_int8(x: torch.Tensor, y: torch.Tensor, weight: torch.Tenso
     """``x.add_(y)``, rounded to its dtype, then ``rms_norm_rows_int8(x, weight, eps)``, in one
     launch. ``x`` is updated in place; its rows must not overlap each other's, nor ``y``'s unless
     ``y`` is ``x``."""
+    if _fast is not None and (got := _fast.quantize(ADD_NORM, x, y, weight, eps)) is not None:
+        return got
     t, n, code = _matrix(x, "x")
     _norm_args(weight, x, n, eps)
     if y.dtype is not x.dtype or y.shape != x.shape or (y.stride(1) != 1 and n > 1):
@@ -151,6 +179,8 @@ def add_rms_norm_rows_int8(x: torch.Tensor, y: torch.Tensor, weight: torch.Tenso
 def silu_mul_int8(gate_up: torch.Tensor) -> Int8Rows:
     """``quantize_rows(F.silu(gate) * up)`` of ``[gate | up]`` rows ``[T, 2N]``, in one launch,
     in float32 up to the 8 bits (``silu_mul`` rounds each factor to the dtype)."""
+    if _fast is not None and (got := _fast.quantize(SILU, gate_up, None, None, 0.0)) is not None:
+        return got
     t, n, code = _matrix(gate_up, "gate_up")
     if n % 2:
         raise ValueError(f"need [gate | up] rows of an even width, got {(t, n)}")
@@ -167,6 +197,8 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
             are copied first where the product runs in tiles.
         out: ``[M, N]`` in ``dtype``, unit column stride (default: a new tensor).
     """
+    if _fast is not None and (got := _fast.linear(x, w, dtype, out)) is not None:
+        return got
     m, k = _codes(x, "x")
     n, kw = _codes(w, "w")
     xq, xs = x
@@ -179,6 +211,8 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
     dev = _lib.require_device(xq, xs, wq, ws)
+    if not _bound:
+        _bind_fast()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return int8_linear(x, w, dtype, out)
@@ -208,6 +242,8 @@ def int8_embedding(table: Int8Rows, ids: torch.Tensor, dtype: torch.dtype) -> to
     """Rows ``ids`` of an 8-bit table as ``dtype``: ``table.q[ids] * table.scale[ids][:, None]``,
     ``[T, N]``, rounded once. ids: int64 ``[T]`` (int32 is accepted and widened); an id outside
     the table gives a row of NaN."""
+    if _fast is not None and (got := _fast.embedding(table, ids, dtype)) is not None:
+        return got
     if ids.dim() != 1 or ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be a [T] int64 or int32 tensor, got {ids.dtype} {tuple(ids.shape)}")
     return _rows_of(table, ids, dtype)
@@ -215,6 +251,8 @@ def int8_embedding(table: Int8Rows, ids: torch.Tensor, dtype: torch.dtype) -> to
 
 def dequantize_rows(rows: Int8Rows, dtype: torch.dtype) -> torch.Tensor:
     """The values that ``rows`` stands for, ``q * scale[:, None]``, in ``dtype``, rounded once."""
+    if _fast is not None and (got := _fast.embedding(rows, None, dtype)) is not None:
+        return got
     return _rows_of(rows, None, dtype)
 
 
@@ -234,6 +272,8 @@ def _rows_of(table: Int8Rows, ids: torch.Tensor | None, dtype: torch.dtype) -> t
         if t > MAX_DIM:
             raise ValueError(f"at most {MAX_DIM} ids, got {t}")
         dev = _lib.require_device(q, scale, ids)
+    if not _bound:
+        _bind_fast()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return _rows_of(table, ids, dtype)
