@@ -304,7 +304,7 @@ int ts_add_rms_norm(const void* x, int64_t x_stride, const float* partial, int k
  * with a = max |v| of the row: q = rint(v * (127 / a)), scale = a / 127 (under a norm both are
  * taken without the row's common factor, which goes into the scale). A row with a < 2^-100
  * (before that factor) gets zeros and scale 0; a row with a NaN or an infinity, or whose sum of
- * squares is past float32, gets zeros and scale NaN.
+ * squares or products with w are past float32, gets zeros and scale NaN.
  * x, y and w share `dtype`; any strides and alignment of theirs. q: 16-byte aligned, q_stride a
  * multiple of 16 and at least N rounded up to 16; bytes of a row past N may be written. y may be
  * x or lie beside it in the same rows; an x whose rows overlap each other's or y's is TS_EINVAL.

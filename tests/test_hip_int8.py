@@ -370,6 +370,23 @@ def test_rows_and_columns_of_length_zero() -> None:
     assert int8_embedding(none, torch.empty(0, dtype=torch.int64, device=DEVICE), torch.float16).shape == (0, 16)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_more_rows_than_one_launch_takes(form: str) -> None:
+    """Over 2^21 rows go in several launches: the rows around the seam, as they are alone."""
+    t, n = (1 << 21) + 5, 8
+    x = torch.randn(t, 2 * n if form == "silu" else n, device=DEVICE, generator=torch.Generator(DEVICE).manual_seed(1)).half()
+    c = {"x": x, "y": torch.randn(t, n, device=DEVICE).half(), "w": torch.ones(n, dtype=torch.float16, device=DEVICE)}
+    seam = slice((1 << 21) - 4, t)
+    part = {k: (v if k == "w" else v[seam].clone()) for k, v in c.items()}
+    before = {k: v.cpu() for k, v in part.items()}
+    got, alone = call(form, c), call(form, part)
+    assert torch.equal(got.q[seam], alone.q) and torch.equal(got.scale[seam], alone.scale)
+    assert torch.equal(c["x"][seam], part["x"])
+    check_rows(form, alone, before)
+    assert bool((got.q.abs().amax(1) == 127).all())
+
+
 # ---- the product -----------------------------------------------------------------------------------
 ODD = [(1, 1, 1), (2, 3, 5), (1, 17, 16), (16, 16, 64), (17, 33, 65), (5, 100, 127), (31, 64, 128), (33, 130, 129),
        (64, 48, 200), (65, 1003, 531), (100, 36, 1531), (128, 128, 256), (129, 257, 255), (255, 70, 1024),
@@ -405,6 +422,21 @@ def test_every_tile_shape_and_last_columns(m: int, n: int) -> None:
         assert same(got, acc * x.scale[:, None] * w.scale), k
         half = int8_linear(x, w, torch.bfloat16)
         assert same(half, (acc * x.scale[:, None] * w.scale).bfloat16()), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("m", "n"), [(1_100_003, 3), (3, 1_100_003), (70_001, 40)])
+def test_many_rows_of_one_side(m: int, n: int) -> None:
+    """Grids past 65535 workgroups along either side."""
+    k = 48
+    g = torch.Generator(DEVICE).manual_seed(m)
+    x = Int8Rows(torch.randint(-128, 128, (m, k), dtype=torch.int8, device=DEVICE, generator=g), torch.rand(m, device=DEVICE))
+    w = Int8Rows(torch.randint(-128, 128, (n, k), dtype=torch.int8, device=DEVICE, generator=g), torch.rand(n, device=DEVICE))
+    acc = x.q.float() @ w.q.float().t()  # integers below 2^24: exact
+    assert same(int8_linear(x, w, torch.float32), acc * x.scale[:, None] * w.scale)
+    odd = Int8Rows(x.q[:, :47], x.scale)  # rows that are not 16-byte aligned from 47 columns on
+    acc = odd.q.float() @ w.q[:, :47].float().t()
+    assert same(int8_linear(odd, Int8Rows(w.q[:, :47].contiguous(), w.scale), torch.float32), acc * x.scale[:, None] * w.scale)
 
 
 @pytest.mark.gpu

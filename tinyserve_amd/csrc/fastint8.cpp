@@ -142,7 +142,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (!pair) return nullptr;
   PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(stride == n ? q : q.narrow(1, 0, n)));
   PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(scale));
-  PyObject* args = PyTuple_Pack(1, pair);
+  PyObject* args = PyTuple_GET_ITEM(pair, 0) && PyTuple_GET_ITEM(pair, 1) ? PyTuple_Pack(1, pair) : nullptr;
   Py_DECREF(pair);
   if (!args) return nullptr;
   PyObject* rows = PyTuple_Type.tp_new(rows_type, args, nullptr);

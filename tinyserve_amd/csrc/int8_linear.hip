@@ -224,7 +224,6 @@ __global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a
 template <typename T, int NTW, int MT>
 static int launch_rows8(const LinearArgs& a, bool aligned, hipStream_t st) {
   const dim3 grid((a.N + 16 * NTW - 1) / (16 * NTW), (a.M + 16 * MT - 1) / (16 * MT)), block(8 * kWave);
-  if (grid.y > 65535) return TS_EUNSUPPORTED;
   if (aligned) hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, true>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, false>), grid, block, 0, st, a);
   return launch_status();
@@ -446,7 +445,7 @@ template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
 static int launch_tiles(const LinearArgs& a, hipStream_t st) {
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
   const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-  if (tm * tn > INT32_MAX) return TS_EUNSUPPORTED;
+  if (tm * tn > 1 << 22) return TS_EUNSUPPORTED;  // 2^31 threads
   hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kCols, kStages>), dim3(static_cast<unsigned>(tm * tn)),
                      dim3(GM * GN * kWave), 0, st, a, static_cast<int>(tm), static_cast<int>(tn));
   return launch_status();
@@ -489,14 +488,16 @@ constexpr RowShape kRowShapes[] = {{1, 1, 0.2f}, {2, 1, 0.3f}, {2, 2, 0.5f}, {4,
 static int pick_kernel(int M, int N, int K) {
   const int cus = compute_units();
   const float k = static_cast<float>(K) / 1024.f;
+  auto groups = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   auto times = [&](int bm, int bn) {  // workgroups per compute unit, one after another
-    const int64_t groups = static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn);
-    return static_cast<float>((groups + cus - 1) / cus);
+    return static_cast<float>((groups(bm, bn) + cus - 1) / cus);
   };
+  constexpr int64_t kMost = 1 << 22;  // workgroups of 512 threads: a launch has fewer than 2^32
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 5; ++i) {
     const TileShape& t = kShapes[i];
+    if (i > 0 && groups(t.bm, t.bn) > kMost) continue;
     const float us = times(t.bm, t.bn) * (t.fixed + t.per_k * k);
     if (i == 0 || us < least) {
       best = i;
@@ -504,19 +505,18 @@ static int pick_kernel(int M, int N, int K) {
     }
   }
   const TileShape& t = kShapes[best];
-  if (static_cast<int64_t>((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn) < cus) least += 0.5f * t.per_k * k;
+  if (groups(t.bm, t.bn) < cus) least += 0.5f * t.per_k * k;
   least += 3.0f;
-  int row = 0;
-  float rows_least = 0.f;
   for (int i = 0; i < 6; ++i) {
     const int bm = 16 * kRowShapes[i].mt, bn = 16 * kRowShapes[i].ntw;
+    if ((M + bm - 1) / bm > 65535 || (N + bn - 1) / bn > kMost) continue;
     const float us = 3.f + times(bm, bn) * (kRowShapes[i].fixed + 0.02f * static_cast<float>(bm + bn) * k);
-    if (i == 0 || us < rows_least) {
-      row = i;
-      rows_least = us;
+    if (us < least) {
+      best = -1 - i;
+      least = us;
     }
   }
-  return rows_least < least ? -1 - row : best;
+  return best;
 }
 
 // Rows for direct-to-LDS loads: 16-byte aligned, readable to a whole 16 columns, and, as rows are addressed

@@ -314,14 +314,23 @@ static int launch_quantize(const QuantArgs& a, hipStream_t st) {
   return launch_status();
 }
 
+// Rows per launch: a launch has fewer than 2^32 threads, up to 1024 of them per row.
+constexpr int kRowsPerLaunch = 1 << 21;
+
 template <typename T>
-static int launch_form(const QuantArgs& a, int form, hipStream_t st) {
-  switch (form) {
-    case kPlain: return launch_quantize<T, kPlain>(a, st);
-    case kNorm: return launch_quantize<T, kNorm>(a, st);
-    case kAddNorm: return launch_quantize<T, kAddNorm>(a, st);
-    default: return launch_quantize<T, kSilu>(a, st);
+static int launch_form(QuantArgs a, int form, hipStream_t st) {
+  for (int left = a.rows; left > 0; left -= kRowsPerLaunch) {
+    a.rows = left < kRowsPerLaunch ? left : kRowsPerLaunch;
+    const int rc = form == kPlain ? launch_quantize<T, kPlain>(a, st) : form == kNorm ? launch_quantize<T, kNorm>(a, st)
+                   : form == kAddNorm ? launch_quantize<T, kAddNorm>(a, st) : launch_quantize<T, kSilu>(a, st);
+    if (rc) return rc;
+    a.x = static_cast<const T*>(a.x) + a.rows * a.xs;
+    a.xo = static_cast<T*>(a.xo) + a.rows * a.xs;
+    a.y = static_cast<const T*>(a.y) + a.rows * a.ys;
+    a.q += a.rows * a.qs;
+    a.scale += a.rows;
   }
+  return 0;
 }
 
 // ---- rows of an 8-bit table -----------------------------------------------------------------
