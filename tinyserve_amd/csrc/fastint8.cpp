@@ -4,8 +4,8 @@
 // subclass, sizes that run after a copy) it returns None before anything is done, and the Python
 // function, whose rules these are, goes on. Without this module built every call goes that way.
 //
-// The launch itself is about 2.8 us of host time. With the checks and allocations: int8_linear 7.8
-// us from Python, add_rms_norm_rows_int8 9.2, dequantize_rows 7.3.
+// Host time of a call, from Python alone and from here (the launch takes about 2.8 us of it):
+// int8_linear 7.8 and 4.2 us, add_rms_norm_rows_int8 9.2 and 5.4, dequantize_rows 7.3 and 4.6.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
