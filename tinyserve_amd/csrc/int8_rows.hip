@@ -137,17 +137,15 @@ struct QuantArgs {
   float eps;
 };
 
-// TPR threads per row, CPT chunks of E elements each; up to 64 threads a workgroup takes 256 / TPR
-// rows, else one.
-template <typename T, int FORM, int TPR, int CPT>
-__global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel(const QuantArgs a) {
+// CPT chunks of E elements per thread. LPR lanes of a wave on one row, a workgroup of 256 threads on
+// 256 / LPR rows; or LPR 0: the whole workgroup, of any number of waves up to 16, on one row.
+template <typename T, int FORM, int LPR, int CPT>
+__global__ __launch_bounds__(LPR ? 256 : 1024) void quantize_rows_kernel(const QuantArgs a) {
   constexpr int E = Pack16<T>::N;
-  constexpr int LPR = TPR < kWave ? TPR : kWave;  // lanes of a wave on one row
-  constexpr int WAVES = TPR / LPR;
-  const int wave = threadIdx.x / kWave;
-  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR : blockIdx.x;
-  const int t = threadIdx.x % TPR;
-  if (WAVES == 1 && row >= a.rows) return;
+  const int wave = threadIdx.x / kWave, TPR = LPR ? LPR : blockDim.x;
+  const int64_t row = LPR ? static_cast<int64_t>(blockIdx.x) * (256 / (LPR ? LPR : 1)) + threadIdx.x / (LPR ? LPR : 1) : blockIdx.x;
+  const int t = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
+  if (LPR && row >= a.rows) return;
   const int N = a.N;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   const T* y = static_cast<const T*>(a.y) + row * a.ys;  // kAddNorm
@@ -194,11 +192,12 @@ __global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel
     }
   }
 
-  top = group_umax<LPR>(top);
-  if constexpr (FORM == kNorm || FORM == kAddNorm) ss = group_sum<LPR>(ss);
-  if constexpr (WAVES > 1) {
-    __shared__ uint32_t tops[WAVES];
-    __shared__ float sums[WAVES];
+  constexpr int kLanes = LPR ? LPR : kWave;
+  top = group_umax<kLanes>(top);
+  if constexpr (FORM == kNorm || FORM == kAddNorm) ss = group_sum<kLanes>(ss);
+  if constexpr (LPR == 0) {
+    __shared__ uint32_t tops[16];
+    __shared__ float sums[16];
     if (threadIdx.x % kWave == 0) {
       tops[wave] = top;
       sums[wave] = ss;
@@ -206,8 +205,7 @@ __global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel
     __syncthreads();
     top = 0;
     ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) {  // in the waves' order in every thread
+    for (int k = 0; k < TPR / kWave; ++k) {  // in the waves' order in every thread
       top = max(top, tops[k]);
       ss += sums[k];
     }
@@ -230,11 +228,11 @@ __global__ __launch_bounds__(TPR <= kWave ? 256 : TPR) void quantize_rows_kernel
 }
 
 // Any row length, one element at a time: rows shorter than one 16-byte vector, and rows longer
-// than a workgroup's registers hold, which are read twice.
+// than a workgroup's registers hold, which are read twice. A workgroup per row.
 template <typename T, int FORM>
 __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs a) {
   const int64_t row = blockIdx.x;
-  const int N = a.N, wave = threadIdx.x / kWave;
+  const int N = a.N, wave = threadIdx.x / kWave, threads = blockDim.x;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   T* xo = static_cast<T*>(a.xo) + row * a.xs;
   const T* y = static_cast<const T*>(a.y) + row * a.ys;
@@ -247,7 +245,7 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
   };
   uint32_t top = 0;
   float ss = 0.f;
-  for (int i = threadIdx.x; i < N; i += 1024) {
+  for (int i = threadIdx.x; i < N; i += threads) {
     float f;
     if constexpr (FORM == kAddNorm) {
       const T s = round_f32<T>(to_f32(xo[i]) + to_f32(y[i]));
@@ -270,14 +268,14 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
   __syncthreads();
   top = 0;
   ss = 0.f;
-  for (int k = 0; k < 16; ++k) {
+  for (int k = 0; k < threads / kWave; ++k) {
     top = max(top, tops[k]);
     ss += sums[k];
   }
   const RowScale r = row_scale<FORM>(top, ss, N, a.eps);
   if (threadIdx.x == 0) a.scale[row] = r.scale;
   int8_t* q = a.q + row * a.qs;
-  for (int i = threadIdx.x; i < N; i += 1024) {
+  for (int i = threadIdx.x; i < N; i += threads) {
     float f;
     if constexpr (FORM == kAddNorm) f = to_f32(xo[i]);
     else f = to_f32(x[i]);
@@ -290,27 +288,35 @@ template <typename T, int FORM>
 static int launch_quantize(const QuantArgs& a, hipStream_t st) {
   constexpr int E = Pack16<T>::N;
   const int chunks = (a.N + E - 1) / E;
-  // Few rows: more threads on each, one or two chunks a thread.
-  const bool few = a.rows < 2 * compute_units();
-#define TS_QUANT(P, C)                                                                                       \
-  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, P, C>),                                                  \
-                     dim3((P) <= kWave ? (a.rows + 256 / (P) - 1) / (256 / (P)) : a.rows), dim3((P) <= kWave ? 256 : (P)), 0, st, a)
-  if (a.N < E || chunks > 4096) hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(1024), 0, st, a);
-  else if (chunks <= 16) TS_QUANT(16, 1);
-  else if (chunks <= 32) TS_QUANT(32, 1);
-  else if (chunks <= 64) TS_QUANT(64, 1);
-  else if (few && chunks <= 256) TS_QUANT(256, 1);
-  else if (few && chunks <= 512) TS_QUANT(256, 2);
-  else if (chunks <= 128) TS_QUANT(64, 2);
-  else if (chunks <= 256) TS_QUANT(64, 4);
-  else if (chunks <= 512) TS_QUANT(256, 2);
-  else if (chunks <= 768) TS_QUANT(256, 3);
-  else if (chunks <= 1024) TS_QUANT(256, 4);
-  else if (chunks <= 1536) TS_QUANT(512, 3);
-  else if (chunks <= 2048) TS_QUANT(512, 4);
-  else if (chunks <= 3072) TS_QUANT(1024, 3);
-  else TS_QUANT(1024, 4);
-#undef TS_QUANT
+  // Wide rows: a workgroup of as many threads as there are chunks, up to 1024, then two to four
+  // chunks a thread. Where one array is read and there is much of it, a thread takes two from 256
+  // chunks on: more loads in flight then pay more than more waves. Measured (us, one and two
+  // chunks): quantising 8192 x 8192 bf16 37.0 and 33.3, 32768 x 2048 39.3 and 32.9, 1024 x 2048 3.67
+  // and 3.72, 32 x 2048 3.18 and 3.32; norm 51.6 and 40.2, 44.5 and 40.4, 4.1 and 4.2, 3.5 and 3.8
+  // (2751 x 2048 7.3 and 7.7, 1024 x 8192 9.9 and 9.4); residual + norm 83.1 and 91.5, 81.3 and 89.5,
+  // 5.8 and 6.3; SiLU 62.1 and 64.0, 59.6 and 62.6, 4.7 and 4.8. From 1025 to 1536 chunks three a
+  // thread: four workgroups of up to 512 threads fill a compute unit, two of 704 do not (4096 x 11008,
+  // two and three: quantising 27.9 and 24.6, SiLU 48.3 and 45.6). Narrow rows: 8192 x 512 in one wave
+  // each, four to a workgroup, 5.1 and 8.6 (quantising; residual + norm), a workgroup each 5.4 and
+  // 8.1; 32768 x 64 in 16 lanes each 4.0 and 6.9, in a wave each 10.5 and 15.1.
+#define TS_NARROW(L)                                                                                                 \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, L, 1>), dim3((a.rows + 256 / (L) - 1) / (256 / (L))), dim3(256), 0, st, a)
+#define TS_WIDE(C)                                                                       \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, 0, C>), dim3(a.rows),                \
+                     dim3(((chunks + (C) - 1) / (C) + kWave - 1) / kWave * kWave), 0, st, a)
+  const int64_t much = FORM == kPlain ? 1 << 18 : FORM == kNorm ? 1 << 20 : INT64_MAX;  // chunks in all
+  const bool two = chunks > 1024 || (chunks >= 256 && static_cast<int64_t>(a.rows) * chunks >= much);
+  if (a.N < E || chunks > 4096)
+    hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(a.N < E ? kWave : 1024), 0, st, a);
+  else if (chunks <= 16) TS_NARROW(16);
+  else if (chunks <= 32) TS_NARROW(32);
+  else if (chunks <= 64) TS_NARROW(64);
+  else if (!two) TS_WIDE(1);
+  else if (chunks <= 1024 || (chunks > 1536 && chunks <= 2048)) TS_WIDE(2);
+  else if (chunks <= 3072) TS_WIDE(3);
+  else TS_WIDE(4);
+#undef TS_NARROW
+#undef TS_WIDE
   return launch_status();
 }
 
