@@ -345,10 +345,11 @@ int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, cons
                    int N, int K, int padded, int dtype, void* stream);
 
 /*
- * Copies M rows of N codes to rows of N rounded up to 16, zeros past N: out 16-byte aligned, its
- * stride a multiple of 16.
+ * Copies the rows of one or two matrices of N codes each (b_rows 0: one) to rows of N rounded up to
+ * 16, zeros past N: outputs 16-byte aligned, their common stride a multiple of 16.
  */
-int ts_int8_pad_rows(const int8_t* q, int64_t q_stride, int8_t* out, int64_t o_stride, int M, int N,
+int ts_int8_pad_rows(const int8_t* a, int64_t a_stride, int8_t* a_out, int a_rows, const int8_t* b,
+                     int64_t b_stride, int8_t* b_out, int b_rows, int64_t o_stride, int N,
                      void* stream);
 
 #ifdef __cplusplus

@@ -207,11 +207,12 @@ def test_c_abi_refuses_before_any_launch() -> None:
                 {"padded": 1, "w": 0x2001}, {"padded": 1, "xs": (1 << 23) + 16}):  # fmt: skip
         assert linear(**{**tiled, **bad}) == -2, bad
 
-    def pad(m=2, n=20, qs=20, os=32, q=0x1000, out=0x2000):  # noqa: ANN001, ANN202
-        return lib.ts_int8_pad_rows(q, qs, out, os, m, n, None)
+    def pad(m=2, m2=2, n=20, qs=20, qs2=20, os=32, q=0x1000, q2=0x3000, out=0x2000, out2=0x4000):  # noqa: ANN001, ANN202
+        return lib.ts_int8_pad_rows(q, qs, out, m, q2, qs2, out2, m2, os, n, None)
 
-    assert pad(m=0) == 0 and pad(n=0) == 0
-    for bad in ({"m": -1}, {"m": big}, {"n": big}, {"qs": -1}, {"os": 16}, {"os": 40}, {"out": 0x2008}, {"q": None}, {"out": None}):
+    assert pad(m=0, m2=0) == 0 and pad(n=0) == 0
+    for bad in ({"m": -1}, {"m2": -1}, {"m": big}, {"m2": big}, {"n": big}, {"qs": -1}, {"qs2": -1}, {"os": 16}, {"os": 40},
+                {"out": 0x2008}, {"out2": 0x4004}, {"q": None}, {"q2": None}, {"out": None}, {"out2": None}):  # fmt: skip
         assert pad(**bad) == -1, bad
 
     def embed(t=2, n=4, rows=5, ts=4, os=4, dtype=1, table=0x1000, scale=0x2000, ids=0x3000, out=0x4000):  # noqa: ANN001, ANN202
@@ -596,6 +597,20 @@ def test_both_host_paths(t: int, n: int, dtype: torch.dtype, host_path: str) -> 
     ids = torch.arange(t - 1, -1, -1)
     for kind in (torch.int64, torch.int32):
         assert torch.equal(int8_embedding(got, ids.to(kind).to(DEVICE), dtype).cpu(), want.flip(0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("xk", "wk"), [(1003, 1003), (1003, 1008), (1008, 1003), (1008, 1008), (1024, 1003)])
+def test_both_host_paths_copy_what_tiles_cannot_read(xk: int, wk: int, host_path: str) -> None:
+    """1003 columns of rows of xk and wk bytes: neither, one or both are copied first."""
+    m, n, k = 700, 900, 1003
+    xb, wb = codes(m, xk, 1).to(DEVICE), codes(n, wk, 2).to(DEVICE)
+    x = Int8Rows(xb[:, :k], scales(m, 3).to(DEVICE))
+    w = Int8Rows(wb[:, :k], scales(n, 4).to(DEVICE))
+    out = torch.full((m, n + 2), 5.0, dtype=torch.bfloat16, device=DEVICE)
+    assert torch.equal(int8_linear(x, w, torch.bfloat16).cpu(), linear_want(x, w, torch.bfloat16))
+    assert torch.equal(int8_linear(x, w, torch.bfloat16, out[:, :n]).cpu(), linear_want(x, w, torch.bfloat16))
+    assert bool((out[:, n:] == 5).all())
 
 
 @pytest.mark.gpu

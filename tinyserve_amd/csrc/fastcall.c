@@ -106,8 +106,8 @@ ENTRY(ts_int8_embedding, 11,
       P(0), L(1), P(2), L(3), P(4), P(5), L(6), I(7), I(8), I(9), P(10))
 ENTRY(ts_int8_linear, 14,
       P(0), L(1), P(2), P(3), L(4), P(5), P(6), L(7), I(8), I(9), I(10), I(11), I(12), P(13))
-ENTRY(ts_int8_pad_rows, 7,
-      P(0), L(1), P(2), L(3), I(4), I(5), P(6))
+ENTRY(ts_int8_pad_rows, 11,
+      P(0), L(1), P(2), I(3), P(4), L(5), P(6), I(7), L(8), I(9), P(10))
 
 #define EACH(X)                                                                     \
   X(ts_decode_split)                                                                \

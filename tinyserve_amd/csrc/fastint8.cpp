@@ -1,8 +1,8 @@
 // The host path of hip_int8's calls without the interpreter: an eager call of a kernel of a few
 // microseconds is bound by it. Takes the tensors, checks them, allocates the results and launches;
 // for whatever it does not take (an argument that is refused, another current device, a tensor
-// subclass, sizes that run after a copy) it returns None before anything is done, and the Python
-// function, whose rules these are, goes on. Without this module built every call goes that way.
+// subclass) it returns None with nothing of the caller's written, and the Python function, whose
+// rules these are, goes on. Without this module built every call goes that way.
 //
 // Host time of a call, from Python alone and from here (the launch takes about 2.8 us of it):
 // int8_linear 7.8 and 4.2 us, add_rms_norm_rows_int8 9.2 and 5.4, dequantize_rows 7.3 and 4.6.
@@ -23,6 +23,7 @@ namespace {
 decltype(&ts_int8_quantize_rows) p_quantize;
 decltype(&ts_int8_embedding) p_embedding;
 decltype(&ts_int8_linear) p_linear;
+decltype(&ts_int8_pad_rows) p_pad;
 PyTypeObject* rows_type;   // Int8Rows
 PyObject* current_stream;  // device index -> the current stream's handle
 
@@ -87,6 +88,13 @@ bool stream_of(const at::Tensor& t, void** out) {
 bool readable(const Rows& r) {
   const int64_t need = (r.k + 15) / 16 * 16, stride = r.q->stride(0);
   return stride >= need && r.q->storage_offset() + (r.m - 1) * stride + need <= static_cast<int64_t>(r.q->storage().nbytes());
+}
+
+// Whether tiles can read the rows (hip_int8._fits).
+bool fits(const Rows& r) {
+  const int64_t stride = r.q->stride(0);
+  return reinterpret_cast<uintptr_t>(r.q->const_data_ptr()) % 16 == 0 && stride % 16 == 0 && stride <= (1 << 23) &&
+         (r.k % 16 == 0 || readable(r));
 }
 
 bool scalar_type(PyObject* o, at::ScalarType* t, int* code) {
@@ -172,14 +180,34 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   void* stream;
   if (!stream_of(*x.q, &stream)) return nullptr;
+  const auto* xp = static_cast<const int8_t*>(x.q->const_data_ptr());
+  const auto* wp = static_cast<const int8_t*>(w.q->const_data_ptr());
+  int64_t xs = x.q->stride(0), ws = w.q->stride(0);
+  auto multiply = [&](int padded) {
+    return p_linear(xp, xs, static_cast<const float*>(x.scale->const_data_ptr()), wp, ws,
+                    static_cast<const float*>(w.scale->const_data_ptr()), out.data_ptr(), out.stride(0), static_cast<int>(m),
+                    static_cast<int>(n), static_cast<int>(k), padded, code, stream);
+  };
   const int padded = k % 16 == 0 || (readable(x) && readable(w));
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = p_linear(static_cast<const int8_t*>(x.q->const_data_ptr()), x.q->stride(0), static_cast<const float*>(x.scale->const_data_ptr()),
-                static_cast<const int8_t*>(w.q->const_data_ptr()), w.q->stride(0),
-                static_cast<const float*>(w.scale->const_data_ptr()), out.data_ptr(), out.stride(0), static_cast<int>(m),
-                static_cast<int>(n), static_cast<int>(k), padded, code, stream);
+  rc = multiply(padded);
   Py_END_ALLOW_THREADS
+  if (rc == TS_EUNSUPPORTED) {  // it runs in tiles, which need aligned rows
+    const int64_t stride = (k + 15) / 16 * 16;
+    at::Tensor xc, wc;
+    const auto options = at::TensorOptions().dtype(at::kChar).device(x.q->device());
+    if (!fits(x)) xc = at::empty({m, stride}, options);
+    if (!fits(w)) wc = at::empty({n, stride}, options);
+    auto* xo = xc.defined() ? static_cast<int8_t*>(xc.data_ptr()) : nullptr;
+    auto* wo = wc.defined() ? static_cast<int8_t*>(wc.data_ptr()) : nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_pad(xp, xs, xo, xo ? static_cast<int>(m) : 0, wp, ws, wo, wo ? static_cast<int>(n) : 0, stride, static_cast<int>(k), stream);
+    if (xo) xp = xo, xs = stride;
+    if (wo) wp = wo, ws = stride;
+    if (!rc) rc = multiply(1);
+    Py_END_ALLOW_THREADS
+  }
   if (rc) Py_RETURN_NONE;
   if (a[3] != Py_None) {
     Py_INCREF(a[3]);
@@ -219,11 +247,11 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(quantize, embedding, linear: the library's addresses; Int8Rows; the stream function)
+// bind(quantize, embedding, linear, pad: the library's addresses; Int8Rows; the stream function)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long q, e, l;
+  unsigned long long q, e, l, p;
   PyObject *type, *stream;
-  if (!PyArg_ParseTuple(args, "KKKOO", &q, &e, &l, &type, &stream)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKOO", &q, &e, &l, &p, &type, &stream)) return nullptr;
   if (!PyType_Check(type) || !PyType_IsSubtype(reinterpret_cast<PyTypeObject*>(type), &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "bind takes a tuple type");
     return nullptr;
@@ -237,6 +265,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   p_quantize = reinterpret_cast<decltype(p_quantize)>(static_cast<uintptr_t>(q));
   p_embedding = reinterpret_cast<decltype(p_embedding)>(static_cast<uintptr_t>(e));
   p_linear = reinterpret_cast<decltype(p_linear)>(static_cast<uintptr_t>(l));
+  p_pad = reinterpret_cast<decltype(p_pad)>(static_cast<uintptr_t>(p));
   Py_RETURN_NONE;
 }
 

@@ -383,27 +383,36 @@ __global__ __launch_bounds__(256) void int8_embedding_kernel(const TableArgs a) 
   }
 }
 
-// Rows copied to a stride of whole 16 bytes, zeros past their ends. One thread per 16 bytes.
-__global__ __launch_bounds__(256) void int8_pad_rows_kernel(const int8_t* __restrict__ q, int64_t qs, int8_t* __restrict__ out,
-                                                            int64_t os, int rows, int N, int per_row) {
-  const int64_t total = static_cast<int64_t>(rows) * per_row;
+// Rows of one matrix, or of two, copied to a stride of whole 16 bytes, zeros past their ends. One
+// thread per 16 bytes.
+struct PadArgs {
+  const int8_t *a, *b;
+  int8_t *a_out, *b_out;
+  int64_t as, bs, os;
+  int a_rows, b_rows, N, per_row;
+};
+
+__global__ __launch_bounds__(256) void int8_pad_rows_kernel(const PadArgs p) {
+  const int64_t total = (static_cast<int64_t>(p.a_rows) + p.b_rows) * p.per_row;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t t = u / per_row;
-    const int i = static_cast<int>(u - t * per_row) * 16;
-    const int8_t* p = q + t * qs + i;
+    const int64_t row = u / p.per_row;
+    const int i = static_cast<int>(u - row * p.per_row) * 16;
+    const bool first = row < p.a_rows;
+    const int64_t t = first ? row : row - p.a_rows;
+    const int8_t* q = (first ? p.a + t * p.as : p.b + t * p.bs) + i;
     union {
       u32x4 raw;
       int8_t b[16];
     } c;
     c.raw = u32x4{0, 0, 0, 0};
-    if (i + 16 <= N) {
-      c.raw = load16_loose(p).raw;
+    if (i + 16 <= p.N) {
+      c.raw = load16_loose(q).raw;
     } else {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (i + e < N) c.b[e] = p[e];
+        if (i + e < p.N) c.b[e] = q[e];
     }
-    *reinterpret_cast<u32x4*>(out + t * os + i) = c.raw;
+    *reinterpret_cast<u32x4*>((first ? p.a_out : p.b_out) + t * p.os + i) = c.raw;
   }
 }
 
@@ -467,15 +476,18 @@ extern "C" int ts_int8_embedding(const int8_t* table, int64_t t_stride, const fl
   }
 }
 
-extern "C" int ts_int8_pad_rows(const int8_t* q, int64_t q_stride, int8_t* out, int64_t o_stride, int M, int N, void* stream) {
+extern "C" int ts_int8_pad_rows(const int8_t* a, int64_t a_stride, int8_t* a_out, int a_rows, const int8_t* b,
+                                int64_t b_stride, int8_t* b_out, int b_rows, int64_t o_stride, int N, void* stream) {
   const int64_t padded = (static_cast<int64_t>(N) + 15) / 16 * 16;
-  if (M < 0 || M > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM || q_stride < 0) return TS_EINVAL;
-  if (o_stride < padded || o_stride % 16 || reinterpret_cast<uintptr_t>(out) % 16) return TS_EINVAL;
-  if (M == 0 || N == 0) return 0;
-  if (!q || !out) return TS_EINVAL;
-  const int per_row = static_cast<int>(padded / 16);
-  const int64_t blocks = (static_cast<int64_t>(M) * per_row + 255) / 256;
+  if (a_rows < 0 || a_rows > TS_INT8_MAX_DIM || b_rows < 0 || b_rows > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM)
+    return TS_EINVAL;
+  if (a_stride < 0 || b_stride < 0 || o_stride < padded || o_stride % 16) return TS_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(a_out) | reinterpret_cast<uintptr_t>(b_out)) % 16) return TS_EINVAL;
+  if ((a_rows == 0 && b_rows == 0) || N == 0) return 0;
+  if ((a_rows > 0 && (!a || !a_out)) || (b_rows > 0 && (!b || !b_out))) return TS_EINVAL;
+  const PadArgs p{a, b, a_out, b_out, a_stride, b_stride, o_stride, a_rows, b_rows, N, static_cast<int>(padded / 16)};
+  const int64_t blocks = ((static_cast<int64_t>(a_rows) + b_rows) * p.per_row + 255) / 256;
   hipLaunchKernelGGL(int8_pad_rows_kernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), q, q_stride, out, o_stride, M, N, per_row);
+                     static_cast<hipStream_t>(stream), p);
   return launch_status();
 }

@@ -63,7 +63,7 @@ def _bind_fast() -> None:
     except ImportError:
         return
     lib = _lib.load()
-    names = ("ts_int8_quantize_rows", "ts_int8_embedding", "ts_int8_linear")
+    names = ("ts_int8_quantize_rows", "ts_int8_embedding", "ts_int8_linear", "ts_int8_pad_rows")
     _fastint8.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), Int8Rows, _stream)
     _fast = _fastint8
 
@@ -75,15 +75,30 @@ def _readable(q: torch.Tensor) -> bool:
     return q.stride(0) >= need and q.storage_offset() + (m - 1) * q.stride(0) + need <= q.untyped_storage().nbytes()
 
 
-def _padded(q: torch.Tensor, dev: int) -> torch.Tensor:
-    """``q``, or where its rows are not 16-byte aligned, readable to a whole 16 columns and at
-    most ``MAX_STRIDE`` apart, a copy of it with rows that are, padded with zeros."""
-    m, k = q.shape
-    if q.data_ptr() % 16 == 0 and q.stride(0) % 16 == 0 and q.stride(0) <= MAX_STRIDE and (k % 16 == 0 or _readable(q)):
-        return q
-    out = _empty((m, (k + 15) // 16 * 16), dtype=_INT8, device=q.device)
-    _lib.call("ts_int8_pad_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), m, k, _stream(dev))
-    return out
+def _fits(q: torch.Tensor) -> bool:
+    """Whether tiles can read ``q``: rows 16-byte aligned, readable to a whole 16 columns and at
+    most ``MAX_STRIDE`` apart."""
+    stride = q.stride(0)
+    return q.data_ptr() % 16 == 0 and stride % 16 == 0 and stride <= MAX_STRIDE and (q.shape[1] % 16 == 0 or _readable(q))
+
+
+def _padded(x: torch.Tensor, w: torch.Tensor, dev: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x`` and ``w``, copied to 16-byte aligned rows padded with zeros where tiles cannot read
+    them; both in one launch."""
+    k = x.shape[1]
+    stride = (k + 15) & ~15
+    args: list[int | None] = []
+    got = []
+    for q in (x, w):
+        if _fits(q):
+            args += [None, 0, None, 0]
+            got.append(q)
+        else:
+            out = _empty((q.shape[0], stride), dtype=_INT8, device=q.device)
+            args += [q.data_ptr(), q.stride(0), out.data_ptr(), q.shape[0]]
+            got.append(out)
+    _lib.call("ts_int8_pad_rows", *args, stride, k, _stream(dev))
+    return got[0], got[1]
 
 
 def _matrix(x: torch.Tensor, what: str) -> tuple[int, int, int]:
@@ -230,7 +245,7 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
         rc = _lib.call_status("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
                               ws.data_ptr(), out.data_ptr(), stride, m, n, k, padded, code, _stream(dev))  # fmt: skip
         if rc == _lib.TS_EUNSUPPORTED:  # it runs in tiles, which need aligned rows
-            xq, wq = _padded(xq, dev), _padded(wq, dev)
+            xq, wq = _padded(xq, wq, dev)
             _lib.call("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
                       ws.data_ptr(), out.data_ptr(), stride, m, n, k, 1, code, _stream(dev))  # fmt: skip
         elif rc:
