@@ -336,13 +336,20 @@ int ts_int8_embedding(const int8_t* table, int64_t t_stride, const float* scale,
  * strides multiples of 16 up to 2^23, and, where K is not a multiple of 16, `padded` non-zero: the
  * caller's word that every row may be read up to K rounded up to 16 (those bytes do not count).
  * Other rows are taken too where the output is small; at sizes that run in tiles they return
- * TS_EUNSUPPORTED before any launch, and ts_int8_pad_rows makes rows that fit. No counterpart in
- * the reference's kernels (F.linear of the decoder layer, model.py:137-179).
+ * TS_EUNSUPPORTED before any launch, and ts_int8_pad_rows makes rows that fit. `workspace`, 16-byte
+ * aligned and owned by this call until it has run, lets K be split over workgroups where the output
+ * is small and K long: ts_int8_linear_workspace() bytes. NULL, or fewer bytes: one workgroup goes
+ * through all of K. No counterpart in the reference's kernels (F.linear of the decoder layer,
+ * model.py:137-179).
  */
 #define TS_INT8_MAX_K 131071
 int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w,
                    int64_t w_stride, const float* w_scale, void* out, int64_t o_stride, int M,
-                   int N, int K, int padded, int dtype, void* stream);
+                   int N, int K, int padded, int dtype, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* Bytes of workspace that ts_int8_linear uses for these sizes on the current device (0: none). */
+int64_t ts_int8_linear_workspace(int M, int N, int K);
 
 /*
  * Copies the rows of one or two matrices of N codes each (b_rows 0: one) to rows of N rounded up to

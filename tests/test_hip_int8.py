@@ -194,12 +194,12 @@ def test_c_abi_refuses_before_any_launch() -> None:
                 {"y": 0x1000 - 14, "t": 1}, {"xs": 16, "ys": 16, "y": 0x1000 + 2 * 16 + 14}):  # fmt: skip
         assert quant(form=2, **bad) == -1, bad
 
-    def linear(m=2, n=3, k=4, xs=4, ws=4, os=3, padded=0, dtype=1, x=0x1000, w=0x2000, out=0x3000, a=0x4000, b=0x5000):  # noqa: ANN001, ANN202
-        return lib.ts_int8_linear(x, xs, a, w, ws, b, out, os, m, n, k, padded, dtype, None)
+    def linear(m=2, n=3, k=4, xs=4, ws=4, os=3, padded=0, dtype=1, x=0x1000, w=0x2000, out=0x3000, a=0x4000, b=0x5000, s=None, sb=0):  # noqa: ANN001, ANN202
+        return lib.ts_int8_linear(x, xs, a, w, ws, b, out, os, m, n, k, padded, dtype, s, sb, None)
 
     assert linear(m=0) == 0 and linear(n=0) == 0
     for bad in ({"m": -1}, {"m": big}, {"n": -1}, {"n": big}, {"k": -1}, {"k": 131072}, {"xs": -1}, {"ws": -1}, {"os": 2},
-                {"x": None}, {"w": None}, {"out": None}, {"a": None}, {"b": None}):  # fmt: skip
+                {"x": None}, {"w": None}, {"out": None}, {"a": None}, {"b": None}, {"s": 0x6008, "sb": 64}, {"sb": -1}):  # fmt: skip
         assert linear(**bad) == -1, bad
     assert linear(dtype=7) == -2
     tiled = {"m": 4000, "n": 4000, "os": 4000, "k": 20, "xs": 32, "ws": 32}  # many rows: aligned and readable to 32 columns, or not taken
@@ -448,6 +448,101 @@ def test_largest_sums_are_exact(value: tuple[int, int]) -> None:
     w = Int8Rows(torch.full((20, k), value[1], dtype=torch.int8, device=DEVICE), torch.ones(20, device=DEVICE))
     want = torch.tensor(float(value[0] * value[1] * k))  # the int32, rounded to float32
     assert bool((int8_linear(x, w, torch.float32).cpu() == want).all())
+
+
+# Products that run in parts of K: 2, 3, 4, 6 and 8 of them, in 128 x 128 tiles but for the last one
+# (256 x 256), with odd outputs and columns.
+PARTS = [(146, 6602, 5805), (3270, 263, 5441), (40, 5460, 13418), (2, 4132, 40592), (2, 911, 104701), (2700, 47, 20001), (136, 5787, 15353)]
+
+
+def test_workspace_of_products() -> None:
+    need = _lib.load().ts_int8_linear_workspace
+    for m, n, k in PARTS:
+        parts, rest = divmod(need(m, n, k), m * ((n + 3) // 4) * 16)
+        assert parts in (2, 3, 4, 6, 8) and rest == 0, (m, n, k)
+    for m, n, k in [(0, 4, 9000), (4, 0, 9000), (-1, 4, 9000), (4, 4, -1), (4, 4, 131072), (4, 4, 0), (16, 16, 4096),
+                    (16, 16, 131071), (8192, 8192, 8192), (1 << 30, 1, 131071), (1, 1 << 30, 131071), (1 << 30, 1 << 30, 131071)]:  # fmt: skip
+        assert need(m, n, k) == 0, (m, n, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("m", "n", "k"), PARTS)
+def test_parts_of_the_columns(m: int, n: int, k: int, dtype: torch.dtype, host_path: str) -> None:
+    x = Int8Rows(codes(m, k, 1, full=True).to(DEVICE), scales(m, 2).to(DEVICE))
+    w = Int8Rows(codes(n, k, 3, full=True).to(DEVICE), scales(n, 4).to(DEVICE))
+    want = linear_want(x, w, dtype)
+    wide = torch.full((m, n + 5), 5.0, dtype=dtype, device=DEVICE)
+    assert torch.equal(int8_linear(x, w, dtype).cpu(), want)
+    int8_linear(x, w, dtype, wide[:, 3 : n + 3])
+    assert torch.equal(wide[:, 3 : n + 3].cpu(), want)
+    assert bool((wide[:, :3] == 5).all()) and bool((wide[:, n + 3 :] == 5).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("m", "n", "k"), [(2, 4132, 40592), (40, 5460, 13424)])
+def test_workspace_given_short_and_none(m: int, n: int, k: int) -> None:
+    """The same bits with the workspace, with a byte less and without; nothing past it is written."""
+    lib = _lib.load()
+    x, w, xs, ws = codes(m, k, 1).to(DEVICE), codes(n, k, 2).to(DEVICE), scales(m, 3).to(DEVICE), scales(n, 4).to(DEVICE)
+    want = linear_want(Int8Rows(x, xs), Int8Rows(w, ws), torch.float32)
+    need = lib.ts_int8_linear_workspace(m, n, k)
+    assert need > 0
+    work = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=DEVICE)
+    for given in (need, need - 1, 0):
+        out = torch.zeros(m, n, device=DEVICE)
+        work.fill_(0x5A)
+        rc = lib.ts_int8_linear(x.data_ptr(), k, xs.data_ptr(), w.data_ptr(), k, ws.data_ptr(), out.data_ptr(), n, m, n, k, 1, _lib.DTYPES[torch.float32],
+                                work.data_ptr() if given else None, given, torch.cuda.current_stream().cuda_stream)  # fmt: skip
+        torch.cuda.synchronize()
+        assert rc == 0
+        assert torch.equal(out.cpu(), want), given
+        assert bool((work[need if given == need else 0 :] == 0x5A).all()), given
+
+
+@pytest.mark.gpu
+def test_parts_captured_and_replayed_between_eager_calls(host_path: str) -> None:
+    """Two captured products in parts and eager ones in turn: each has its own sums."""
+    sets = []
+    for m, n, k in ((2, 911, 104701), (40, 5460, 13418)):
+        x = Int8Rows(codes(m, k, 1).to(DEVICE), scales(m, 2).to(DEVICE))
+        w = Int8Rows(codes(n, k, 3).to(DEVICE), scales(n, 4).to(DEVICE))
+        sets.append((x, w, torch.empty(m, n, device=DEVICE)))
+    for x, w, out in sets:
+        int8_linear(x, w, torch.float32, out)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in sets]
+    for g, (x, w, out) in zip(graphs, sets, strict=True):
+        with torch.cuda.graph(g):
+            int8_linear(x, w, torch.float32, out)
+    for round_ in range(3):
+        for i, (x, w, out) in enumerate(sets):
+            x.q.copy_(codes(*x.q.shape, 10 * round_ + i))
+            out.zero_()
+        for g in graphs:
+            g.replay()
+        eager = [int8_linear(x, w, torch.float32) for x, w, _ in sets]
+        torch.cuda.synchronize()
+        for (x, w, out), e in zip(sets, eager, strict=True):
+            want = linear_want(x, w, torch.float32)
+            assert torch.equal(out.cpu(), want) and torch.equal(e.cpu(), want)
+
+
+@pytest.mark.gpu
+def test_parts_on_two_streams_at_once(host_path: str) -> None:
+    m, n, k = 2, 911, 104701
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = [(Int8Rows(codes(m, k, i).to(DEVICE), scales(m, i).to(DEVICE)), Int8Rows(codes(n, k, 9 + i).to(DEVICE), scales(n, 9 + i).to(DEVICE))) for i in range(2)]  # fmt: skip
+    torch.cuda.synchronize()
+    outs: list[list[torch.Tensor]] = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(int8_linear(*sets[i], torch.bfloat16))
+    torch.cuda.synchronize()
+    for (x, w), got in zip(sets, outs, strict=True):
+        want = linear_want(x, w, torch.bfloat16)
+        assert all(torch.equal(o.cpu(), want) for o in got)
 
 
 @pytest.mark.gpu

@@ -76,7 +76,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ts_add_rms_norm": (_i, [_vp, _i64, _vp, _i, _vp, _vp, _i64, _vp, _i, _i64, _i, _i, _f, _i, _vp]),
     "ts_int8_quantize_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _f, _i, _i, _vp]),
     "ts_int8_embedding": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _vp]),
-    "ts_int8_linear": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "ts_int8_linear": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
+    "ts_int8_linear_workspace": (_i64, [_i, _i, _i]),
     "ts_int8_pad_rows": (_i, [_vp, _i64, _vp, _i, _vp, _i64, _vp, _i, _i64, _i, _vp]),
 }  # fmt: skip
 

@@ -104,8 +104,8 @@ ENTRY(ts_int8_quantize_rows, 14,
       P(0), P(1), P(2), P(3), P(4), I(5), I(6), L(7), L(8), L(9), F(10), I(11), I(12), P(13))
 ENTRY(ts_int8_embedding, 11,
       P(0), L(1), P(2), L(3), P(4), P(5), L(6), I(7), I(8), I(9), P(10))
-ENTRY(ts_int8_linear, 14,
-      P(0), L(1), P(2), P(3), L(4), P(5), P(6), L(7), I(8), I(9), I(10), I(11), I(12), P(13))
+ENTRY(ts_int8_linear, 16,
+      P(0), L(1), P(2), P(3), L(4), P(5), P(6), L(7), I(8), I(9), I(10), I(11), I(12), P(13), L(14), P(15))
 ENTRY(ts_int8_pad_rows, 11,
       P(0), L(1), P(2), I(3), P(4), L(5), P(6), I(7), L(8), I(9), P(10))
 

@@ -23,6 +23,7 @@ namespace {
 decltype(&ts_int8_quantize_rows) p_quantize;
 decltype(&ts_int8_embedding) p_embedding;
 decltype(&ts_int8_linear) p_linear;
+decltype(&ts_int8_linear_workspace) p_workspace;
 decltype(&ts_int8_pad_rows) p_pad;
 PyTypeObject* rows_type;   // Int8Rows
 PyObject* current_stream;  // device index -> the current stream's handle
@@ -183,10 +184,14 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const auto* xp = static_cast<const int8_t*>(x.q->const_data_ptr());
   const auto* wp = static_cast<const int8_t*>(w.q->const_data_ptr());
   int64_t xs = x.q->stride(0), ws = w.q->stride(0);
+  const int64_t need = p_workspace(static_cast<int>(m), static_cast<int>(n), static_cast<int>(k));
+  at::Tensor sums;
+  if (need) sums = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(x.q->device()));
+  void* const sums_at = need ? sums.data_ptr() : nullptr;
   auto multiply = [&](int padded) {
     return p_linear(xp, xs, static_cast<const float*>(x.scale->const_data_ptr()), wp, ws,
                     static_cast<const float*>(w.scale->const_data_ptr()), out.data_ptr(), out.stride(0), static_cast<int>(m),
-                    static_cast<int>(n), static_cast<int>(k), padded, code, stream);
+                    static_cast<int>(n), static_cast<int>(k), padded, code, sums_at, need, stream);
   };
   const int padded = k % 16 == 0 || (readable(x) && readable(w));
   int rc;
@@ -247,11 +252,11 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(quantize, embedding, linear, pad: the library's addresses; Int8Rows; the stream function)
+// bind(quantize, embedding, linear, its workspace, pad: the library's addresses; Int8Rows; the stream function)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long q, e, l, p;
+  unsigned long long q, e, l, s, p;
   PyObject *type, *stream;
-  if (!PyArg_ParseTuple(args, "KKKKOO", &q, &e, &l, &p, &type, &stream)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKOO", &q, &e, &l, &s, &p, &type, &stream)) return nullptr;
   if (!PyType_Check(type) || !PyType_IsSubtype(reinterpret_cast<PyTypeObject*>(type), &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "bind takes a tuple type");
     return nullptr;
@@ -265,6 +270,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   p_quantize = reinterpret_cast<decltype(p_quantize)>(static_cast<uintptr_t>(q));
   p_embedding = reinterpret_cast<decltype(p_embedding)>(static_cast<uintptr_t>(e));
   p_linear = reinterpret_cast<decltype(p_linear)>(static_cast<uintptr_t>(l));
+  p_workspace = reinterpret_cast<decltype(p_workspace)>(static_cast<uintptr_t>(s));
   p_pad = reinterpret_cast<decltype(p_pad)>(static_cast<uintptr_t>(p));
   Py_RETURN_NONE;
 }

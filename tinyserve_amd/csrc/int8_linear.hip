@@ -9,6 +9,8 @@
 //
 // No kernel of the reference corresponds: it stands for F.linear of the decoder layer
 // (src/tinyserve/model.py:137-179) where the weights are kept in 8 bits.
+#include <type_traits>
+
 #include "common.h"
 
 namespace ts {
@@ -26,6 +28,7 @@ struct LinearArgs {
   void* out;
   int M, N, K;
   int64_t xs, ws, os;
+  int per;  // tile columns per part of K, where K is split over workgroups
 };
 
 // 16 codes at any address (gfx950 takes unaligned vector loads).
@@ -115,15 +118,38 @@ __device__ __forceinline__ i32x4 byte_mask(int lo, int hi) {
   return m;
 }
 
+// Division of 0 .. 2^22 by a number of the launch, 1 .. 2^22: a product with ceil(2^s / by) for s = 22 +
+// ceil(log2(by)), in the scalar unit. (The compiler's division takes 0.1 us of 64 x 1024 x 2048's 3.7.)
+struct Divisor {
+  int by, shift;
+  uint32_t factor;
+  explicit Divisor(int d) : by(d), shift(0), factor(1u << 23) {
+    int log = 0;
+    while ((1 << log) < d) ++log;
+    if (d > 1) {
+      shift = log - 1;
+      factor = static_cast<uint32_t>(((1ull << (22 + log)) + d - 1) / d);
+    }
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    return static_cast<int>(__umulhi(static_cast<uint32_t>(n) << 9, factor) >> shift);
+  }
+};
+
 template <typename T, int NTW, int MT, bool kAligned>
-__global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a) {
+__global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a, const Divisor tiles_m) {
   constexpr int KP = 8, BN = 16 * NTW, BM = 16 * MT, L = (BM + BN) / 8;  // L: loads per unit
   constexpr int RED = BN + 4;  // padded row of the part sums, 16-byte aligned
   constexpr int kUnit = (BM + BN) * 128, kRing = KP * kUnit, kSums = KP * BM * RED * 4;
   __shared__ __attribute__((aligned(16))) int8_t lds[kRing > kSums ? kRing : kSums];
   const int tid = threadIdx.x, lane = tid % kWave;
   const int kp = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
+  // Workgroups go round-robin over the 8 XCDs: those of the same rows of W run on one of them, which
+  // reads W once (22 x 3968 x 6656 11.0 us by a grid of two dimensions, 7.9 so; 54 x 1856 x 25664 in
+  // one part 32.2 and 20.6).
+  const int xcd = blockIdx.x % 8, per = gridDim.x / 8, more = gridDim.x % 8;
+  const int tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
+  const int tn = tiles_m.quotient(tile), n0 = tn * BN, m0 = (tile - tn * tiles_m.by) * BM;
   int8_t* const slot = lds + kp * kUnit;
 
   // Load j fills rows 8 j .. of a unit, of W and then of x; rows past the ends repeat the last one
@@ -223,9 +249,11 @@ __global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a
 
 template <typename T, int NTW, int MT>
 static int launch_rows8(const LinearArgs& a, bool aligned, hipStream_t st) {
-  const dim3 grid((a.N + 16 * NTW - 1) / (16 * NTW), (a.M + 16 * MT - 1) / (16 * MT)), block(8 * kWave);
-  if (aligned) hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, false>), grid, block, 0, st, a);
+  const int64_t tn = (a.N + 16 * NTW - 1) / (16 * NTW), tm = (a.M + 16 * MT - 1) / (16 * MT);
+  if (tm * tn > 1 << 22) return TS_EUNSUPPORTED;  // 2^31 threads
+  const dim3 grid(static_cast<unsigned>(tm * tn)), block(8 * kWave);
+  if (aligned) hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, true>), grid, block, 0, st, a, Divisor(static_cast<int>(tm)));
+  else hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, false>), grid, block, 0, st, a, Divisor(static_cast<int>(tm)));
   return launch_status();
 }
 
@@ -243,8 +271,12 @@ static int launch_rows8(const LinearArgs& a, bool aligned, hipStream_t st) {
 // Columns past the last whole tile: one more tile that ends where the rows (rounded up to 16
 // columns) end; the columns of it that the tile before held, or that lie past K, are masked out
 // of W's operand in registers.
+//
+// T int32_t: a part of K per workgroup, `per` tiles of it, the sums of part p as they are at row
+// p * M + m of `out`.
 template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
-__global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(LinearArgs a, int tiles_m, int tiles_n) {
+  constexpr bool kPart = std::is_same_v<T, int32_t>;
   constexpr int kWaves = GM * GN, kThreads = kWaves * kWave;
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
   constexpr int kUnits = kCols / 16, kSteps = kCols / 32, RPL = kWave / kUnits;  // RPL: rows per load
@@ -266,8 +298,16 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
   // bands of 4 tiles of x, so that the tiles running on it share rows of x and W in its L2.
   int tm, tn;
   {
-    const int total = tiles_m * tiles_n, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
-    const int t = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    const int total = gridDim.x, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
+    int t = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    if constexpr (kPart) {
+      const int part = t / (tiles_m * tiles_n), k0 = part * a.per * kCols;
+      t -= part * tiles_m * tiles_n;
+      a.x += k0;
+      a.w += k0;
+      a.K = min(a.K - k0, a.per * kCols);
+      a.out = static_cast<T*>(a.out) + part * a.M * a.os;
+    }
     const int band = t / (4 * tiles_n), first = band * 4, high = min(4, tiles_m - first);
     const int in = t - band * 4 * tiles_n;
     tm = first + in % high;
@@ -275,8 +315,8 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
   }
   const int m0 = tm * BM, n0 = tn * BN;
   // Each thread keeps a few of the tile's scales until the end.
-  constexpr int kScales = (BM + BN + kThreads - 1) / kThreads;
-  float scale[kScales];
+  constexpr int kScales = kPart ? 0 : (BM + BN + kThreads - 1) / kThreads;
+  float scale[kScales + 1];
 #pragma unroll
   for (int i = 0; i < kScales; ++i) {
     const int c = threadIdx.x + i * kThreads;
@@ -408,16 +448,22 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
   constexpr int E = Pack16<T>::N, VPR = 32 * NW / E;  // vectors per row
 #pragma unroll
   for (int u = 0; u < MW; ++u) {
-    const float s = scales[BN + (wm * MW + u) * 32 + lane % 32];
+    float s = 1.f;
+    if constexpr (!kPart) s = scales[BN + (wm * MW + u) * 32 + lane % 32];
 #pragma unroll
     for (int t = 0; t < NW; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = t * 32 + j * 8 + lane / 32 * 4;
-        const f32x4 sw = *reinterpret_cast<const f32x4*>(scales + wn * 32 * NW + c);
         typename Vec4<T>::V y;
+        if constexpr (kPart) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = round_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * sw[i]);
+          for (int i = 0; i < 4; ++i) y[i] = acc[t][u][j * 4 + i];
+        } else {
+          const f32x4 sw = *reinterpret_cast<const f32x4*>(scales + wn * 32 * NW + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = round_f32<T>(static_cast<float>(acc[t][u][j * 4 + i]) * s * sw[i]);
+        }
         *reinterpret_cast<typename Vec4<T>::V*>(mine + (lane % 32) * kRow + c * sizeof(T)) = y;
       }
     __builtin_amdgcn_wave_barrier();
@@ -441,6 +487,19 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(const Lin
   }
 }
 
+// The sums of the parts of K, and the outputs of them: four to a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_parts_kernel(const LinearArgs a, const int32_t* sums, int parts, int quads) {
+  const int i = blockIdx.x * 256 + threadIdx.x, m = i / quads, n = (i - m * quads) * 4;
+  if (m >= a.M) return;
+  const int64_t each = static_cast<int64_t>(a.M) * quads * 4;
+  const int32_t* p = sums + static_cast<int64_t>(i) * 4;
+  i32x4 v = *reinterpret_cast<const i32x4*>(p);
+#pragma unroll 4
+  for (int k = 1; k < parts; ++k) v += *reinterpret_cast<const i32x4*>(p + k * each);
+  store_outputs<T>(a, m, n, v);
+}
+
 template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
 static int launch_tiles(const LinearArgs& a, hipStream_t st) {
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
@@ -448,6 +507,21 @@ static int launch_tiles(const LinearArgs& a, hipStream_t st) {
   if (tm * tn > 1 << 22) return TS_EUNSUPPORTED;  // 2^31 threads
   hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kCols, kStages>), dim3(static_cast<unsigned>(tm * tn)),
                      dim3(GM * GN * kWave), 0, st, a, static_cast<int>(tm), static_cast<int>(tn));
+  return launch_status();
+}
+
+template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
+static int launch_parts(LinearArgs a, int parts, int32_t* sums, hipStream_t st) {
+  constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
+  const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN, quads = (a.N + 3) / 4;
+  LinearArgs part = a;
+  part.out = sums;
+  part.os = quads * 4;
+  part.per = ((a.K + kCols - 1) / kCols + parts - 1) / parts;
+  hipLaunchKernelGGL((int8_tile_kernel<int32_t, MW, NW, GM, GN, kCols, kStages>), dim3(tm * tn * parts),
+                     dim3(GM * GN * kWave), 0, st, part, tm, tn);
+  if (const int rc = launch_status()) return rc;
+  hipLaunchKernelGGL(int8_parts_kernel<T>, dim3((a.M * quads + 255) / 256), dim3(256), 0, st, a, sums, parts, quads);
   return launch_status();
 }
 
@@ -463,11 +537,11 @@ struct TileShape {
   float fixed, per_k;
 };
 constexpr TileShape kShapes[] = {
-    {256, 256, 6.4f, 10.1f},  // 8 waves of 128 x 64
-    {192, 128, 3.6f, 5.0f},   // 4 waves of 96 x 64, two workgroups per CU
-    {128, 128, 2.2f, 4.4f},   // 8 waves of 64 x 32, three stages
-    {64, 128, 1.3f, 2.3f},    // 4 waves of 32 x 64, three stages, two workgroups per CU
-    {64, 64, 1.0f, 1.6f},     // 4 waves of 32 x 32, four stages, two workgroups per CU
+    {256, 256, 6.4f, 10.0f},  // 8 waves of 128 x 64
+    {192, 128, 3.2f, 4.4f},   // 4 waves of 96 x 64, two workgroups per CU
+    {128, 128, 2.4f, 4.4f},   // 8 waves of 64 x 32, three stages
+    {64, 128, 1.9f, 2.55f},   // 4 waves of 32 x 64, three stages, two workgroups per CU
+    {64, 64, 0.8f, 1.6f},     // 4 waves of 32 x 32, four stages, two workgroups per CU
 };
 
 // Row kernels, as 16-row tiles of W and of x per workgroup, with what a workgroup takes beside its
@@ -476,47 +550,83 @@ struct RowShape {
   int ntw, mt;
   float fixed;
 };
-constexpr RowShape kRowShapes[] = {{1, 1, 0.2f}, {2, 1, 0.3f}, {2, 2, 0.5f}, {4, 1, 0.5f}, {4, 2, 1.2f}, {4, 4, 2.5f}};
+constexpr RowShape kRowShapes[] = {{1, 1, 0.2f}, {2, 1, 0.25f}, {2, 2, 0.5f}, {4, 1, 0.7f}, {4, 2, 1.2f}, {4, 4, 2.2f}};
 
-// Which kernel: a tile shape (0 ..), or a row shape (-1 - index). Both are priced in us. A row
-// kernel takes, beside its start, what its workgroups bring into one compute unit, at about 50
-// KB a us (measured at 64 x 8192 x 8192, in the order of the
-// table but for the second: 41.8, 27.7, 26.8, 21.2, 26.7 us, and at 64 x 4096 x 1024 5.2, 4.6,
-// 4.7, 5.2, 6.5). Tiles that do not fill the chip wait for W: half as much again per column.
-// Measured, row kernel against tiles: 128 x 2048 x 4096 6.7 and 10.6, 64 x 8192 x 8192 21.2 and
-// 26.7, 128 x 8192 x 8192 25.6 and 26.4, 64 x 16384 x 2048 11.8 and 9.6, 64 x 151936 x 1024 62 and 35.
-static int pick_kernel(int M, int N, int K) {
+// What runs: a tile shape (0 ..) or a row shape (-1 - index), and the parts of K that workgroups of
+// their own take.
+struct Pick {
+  int kernel, parts;
+};
+
+// Both kinds are priced in us, by constants fitted to 357 products of 1 .. 8192 rows and 64 .. 28672
+// columns and outputs, each timed with every kernel: the pick takes 0.9% longer than the best of
+// them on average, 24% at most. A row kernel takes, beside its start, what its workgroups bring
+// into one compute unit, at about 55 KB a us. Tiles that do not fill the chip wait for W: half as
+// much again per column. Past 4096 columns loads come slower (`deep`): fewer of them find their
+// lines in L2. Measured, row kernel against tiles: 128 x 2048 x 4096 6.5 and 10.6, 64 x 8192 x 8192
+// 20.9 and 26.7, 64 x 16384 x 2048 11.8 and 9.6, 64 x 151936 x 1024 62 and 35.
+//
+// K split over workgroups: few tiles over many columns leave compute units without one, or with one
+// where others have two. It costs a second launch and the sums' way through memory (5.5 us, 3.2
+// TB/s). Measured, us without and with: 384 x 4096 x 11008 46.6 and 36.8 (128 x 128, two parts),
+// 297 x 4288 x 15680 68 and 47 (the same), 1257 x 3392 x 27328 247 and 144 (256 x 256, three), 137 x
+// 6464 x 18112 74 and 50 (256 x 256, eight); but 256 x 4096 x 4096 12.3 and 16.4, 1024 x 8192 x 8192
+// 83.7 and 85.1. Parts of the other shapes would add 0.2% over all the products.
+static Pick pick_kernel(int M, int N, int K, bool may_split) {
   const int cus = compute_units();
-  const float k = static_cast<float>(K) / 1024.f;
+  const float k = static_cast<float>(K) / 1024.f, deep = k > 4.f ? k - 4.f : 0.f;
   auto groups = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  auto times = [&](int bm, int bn) {  // workgroups per compute unit, one after another
-    return static_cast<float>((groups(bm, bn) + cus - 1) / cus);
-  };
+  auto times = [&](int64_t g) { return static_cast<float>((g + cus - 1) / cus); };  // workgroups per compute unit, one after another
   constexpr int64_t kMost = 1 << 22;  // workgroups of 512 threads: a launch has fewer than 2^32
-  int best = 0;
+  Pick best{0, 1};
   float least = 0.f;
   for (int i = 0; i < 5; ++i) {
     const TileShape& t = kShapes[i];
-    if (i > 0 && groups(t.bm, t.bn) > kMost) continue;
-    const float us = times(t.bm, t.bn) * (t.fixed + t.per_k * k);
+    const int64_t g = groups(t.bm, t.bn);
+    if (i > 0 && g > kMost) continue;
+    const float us = times(g) * (t.fixed + t.per_k * k);
     if (i == 0 || us < least) {
-      best = i;
+      best.kernel = i;
       least = us;
     }
   }
-  const TileShape& t = kShapes[best];
-  if (groups(t.bm, t.bn) < cus) least += 0.5f * t.per_k * k;
-  least += 3.0f;
+  const TileShape& t = kShapes[best.kernel];
+  const int64_t g = groups(t.bm, t.bn);
+  least += 3.0f + times(g) * t.per_k * 1.2f * deep;
+  if (g < cus) least += 0.5f * t.per_k * k;
   for (int i = 0; i < 6; ++i) {
     const int bm = 16 * kRowShapes[i].mt, bn = 16 * kRowShapes[i].ntw;
-    if ((M + bm - 1) / bm > 65535 || (N + bn - 1) / bn > kMost) continue;
-    const float us = 3.f + times(bm, bn) * (kRowShapes[i].fixed + 0.02f * static_cast<float>(bm + bn) * k);
+    if (groups(bm, bn) > kMost) continue;
+    const float us = 3.f + times(groups(bm, bn)) * (kRowShapes[i].fixed + 0.018f * static_cast<float>(bm + bn) * (k + 0.3f * deep));
     if (us < least) {
-      best = -1 - i;
+      best.kernel = -1 - i;
       least = us;
+    }
+  }
+  if (!may_split || deep == 0.f) return best;
+  const int columns = (K + 127) / 128;
+  const float outputs = static_cast<float>(M) * static_cast<float>(N);
+  for (int i : {0, 2}) {
+    const TileShape& t = kShapes[i];
+    for (int parts : {2, 3, 4, 6, 8}) {
+      const int per = (columns + parts - 1) / parts;
+      const int64_t g = groups(t.bm, t.bn) * parts;
+      if ((parts - 1) * per >= columns || g > 4 * cus) continue;  // a part would be empty; nothing to fill
+      if (g < cus / 4) continue;  // 16 x 16 x 131056 in 8 parts 57, as one workgroup of the row kernel 50
+      const float us = 8.5f + times(g) * (t.fixed + 1.2f * t.per_k * static_cast<float>(per) / 8.f) +
+                       outputs * 8.f * static_cast<float>(parts) / 3.2e6f;
+      if (us < least) {
+        best = {i, parts};
+        least = us;
+      }
     }
   }
   return best;
+}
+
+// Bytes of the sums of `parts` parts.
+static int64_t parts_bytes(int M, int N, int parts) {
+  return parts > 1 ? static_cast<int64_t>(parts) * M * ((static_cast<int64_t>(N) + 3) / 4 * 16) : 0;
 }
 
 // Rows for direct-to-LDS loads: 16-byte aligned, readable to a whole 16 columns, and, as rows are addressed
@@ -527,11 +637,18 @@ static bool rows_fit(const LinearArgs& a, bool padded) {
 }
 
 template <typename T>
-static int launch_linear(const LinearArgs& a, bool padded, hipStream_t st) {
+static int launch_linear(const LinearArgs& a, bool padded, int32_t* sums, int64_t bytes, hipStream_t st) {
   const bool aligned = rows_fit(a, padded);
-  const int kernel = pick_kernel(a.M, a.N, a.K);
-  if (kernel >= 0 && !aligned) return TS_EUNSUPPORTED;
-  switch (kernel) {
+  Pick pick = pick_kernel(a.M, a.N, a.K, sums != nullptr);
+  if (parts_bytes(a.M, a.N, pick.parts) > bytes) pick = pick_kernel(a.M, a.N, a.K, false);
+  if (pick.kernel >= 0 && !aligned) return TS_EUNSUPPORTED;
+  if (pick.parts > 1) {
+    switch (pick.kernel) {
+      case 0: return launch_parts<T, 4, 2, 2, 4, 128, 2>(a, pick.parts, sums, st);
+      default: return launch_parts<T, 2, 1, 2, 4, 128, 3>(a, pick.parts, sums, st);
+    }
+  }
+  switch (pick.kernel) {
     case -1: return launch_rows8<T, 1, 1>(a, aligned, st);
     case -2: return launch_rows8<T, 2, 1>(a, aligned, st);
     case -3: return launch_rows8<T, 2, 2>(a, aligned, st);
@@ -550,19 +667,26 @@ static int launch_linear(const LinearArgs& a, bool padded, hipStream_t st) {
 
 using namespace ts;
 
+extern "C" int64_t ts_int8_linear_workspace(int M, int N, int K) {
+  if (M <= 0 || M > TS_INT8_MAX_DIM || N <= 0 || N > TS_INT8_MAX_DIM || K < 0 || K > TS_INT8_MAX_K) return 0;
+  return parts_bytes(M, N, pick_kernel(M, N, K, true).parts);
+}
+
 extern "C" int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                               const float* w_scale, void* out, int64_t o_stride, int M, int N, int K, int padded,
-                              int dtype, void* stream) {
+                              int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (M < 0 || M > TS_INT8_MAX_DIM || N < 0 || N > TS_INT8_MAX_DIM || K < 0 || K > TS_INT8_MAX_K || x_stride < 0 || w_stride < 0) return TS_EINVAL;
   if (M > 1 && o_stride < N) return TS_EINVAL;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < 0) return TS_EINVAL;
   if (dtype < TS_F32 || dtype > TS_BF16) return TS_EUNSUPPORTED;
   if (M == 0 || N == 0) return 0;
   if (!out || !x_scale || !w_scale || (K > 0 && (!x || !w))) return TS_EINVAL;
-  const LinearArgs a{x, w, x_scale, w_scale, out, M, N, K, x_stride, w_stride, o_stride};
+  const LinearArgs a{x, w, x_scale, w_scale, out, M, N, K, x_stride, w_stride, o_stride, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
+  auto* sums = static_cast<int32_t*>(workspace);
   switch (dtype) {
-    case TS_F32: return launch_linear<float>(a, padded != 0, st);
-    case TS_F16: return launch_linear<f16>(a, padded != 0, st);
-    default: return launch_linear<bf16>(a, padded != 0, st);
+    case TS_F32: return launch_linear<float>(a, padded != 0, sums, workspace_bytes, st);
+    case TS_F16: return launch_linear<f16>(a, padded != 0, sums, workspace_bytes, st);
+    default: return launch_linear<bf16>(a, padded != 0, sums, workspace_bytes, st);
   }
 }

@@ -63,7 +63,7 @@ def _bind_fast() -> None:
     except ImportError:
         return
     lib = _lib.load()
-    names = ("ts_int8_quantize_rows", "ts_int8_embedding", "ts_int8_linear", "ts_int8_pad_rows")
+    names = ("ts_int8_quantize_rows", "ts_int8_embedding", "ts_int8_linear", "ts_int8_linear_workspace", "ts_int8_pad_rows")
     _fastint8.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), Int8Rows, _stream)
     _fast = _fastint8
 
@@ -242,12 +242,15 @@ def int8_linear(x: Int8Rows, w: Int8Rows, dtype: torch.dtype, out: torch.Tensor 
         stride = out.stride(0)
     if m and n:
         padded = k % 16 == 0 or (_readable(xq) and _readable(wq))
+        need = _lib.load().ts_int8_linear_workspace(m, n, k)
+        workspace = _empty(need, dtype=torch.uint8, device=xq.device) if need else None  # kept until both launches
+        sums = None if workspace is None else workspace.data_ptr()
         rc = _lib.call_status("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-                              ws.data_ptr(), out.data_ptr(), stride, m, n, k, padded, code, _stream(dev))  # fmt: skip
+                              ws.data_ptr(), out.data_ptr(), stride, m, n, k, padded, code, sums, need, _stream(dev))  # fmt: skip
         if rc == _lib.TS_EUNSUPPORTED:  # it runs in tiles, which need aligned rows
             xq, wq = _padded(xq, wq, dev)
             _lib.call("ts_int8_linear", xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
-                      ws.data_ptr(), out.data_ptr(), stride, m, n, k, 1, code, _stream(dev))  # fmt: skip
+                      ws.data_ptr(), out.data_ptr(), stride, m, n, k, 1, code, sums, need, _stream(dev))  # fmt: skip
         elif rc:
             raise ValueError(f"ts_int8_linear: {_lib.load().ts_strerror(rc).decode()}")
     return out
