@@ -56,7 +56,7 @@ __device__ __forceinline__ Pack16<T> load_chunk(const T* row, int i, int N) {
 // The exponent is taken from g cut to where 2^t is finite: below -88.7 the result, under 1e-36 in
 // magnitude, is -88.7's; the last term makes an infinity or a NaN in g a NaN.
 // The hardware's exp2 and reciprocal are within one unit in the last place; expf and a correctly
-// rounded quotient made the kernel wait for its arithmetic (8192 x 8192 bf16 82 us, now 68).
+// rounded quotient made the kernel wait for its arithmetic (8192 x 8192 bf16 82 us, then 68).
 __device__ __forceinline__ float silu(float g) {
   constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - (float)log2(e)
   constexpr float kLn2 = 0.693147180559945f;
