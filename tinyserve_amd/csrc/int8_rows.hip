@@ -304,16 +304,17 @@ static int launch_quantize(const QuantArgs& a, hipStream_t st) {
 #define TS_WIDE(C)                                                                       \
   hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, 0, C>), dim3(a.rows),                \
                      dim3(((chunks + (C) - 1) / (C) + kWave - 1) / kWave * kWave), 0, st, a)
+  constexpr int kMost = 1024;  // threads of a workgroup
   const int64_t much = FORM == kPlain ? 1 << 18 : FORM == kNorm ? 1 << 20 : INT64_MAX;  // chunks in all
-  const bool two = chunks > 1024 || (chunks >= 256 && static_cast<int64_t>(a.rows) * chunks >= much);
-  if (a.N < E || chunks > 4096)
-    hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(a.N < E ? kWave : 1024), 0, st, a);
+  const bool two = chunks > kMost || (chunks >= 256 && static_cast<int64_t>(a.rows) * chunks >= much);
+  if (a.N < E || chunks > 4 * kMost)
+    hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(a.N < E ? kWave : kMost), 0, st, a);
   else if (chunks <= 16) TS_NARROW(16);
   else if (chunks <= 32) TS_NARROW(32);
   else if (chunks <= 64) TS_NARROW(64);
   else if (!two) TS_WIDE(1);
-  else if (chunks <= 1024 || (chunks > 1536 && chunks <= 2048)) TS_WIDE(2);
-  else if (chunks <= 3072) TS_WIDE(3);
+  else if (chunks <= kMost || (chunks > kMost * 3 / 2 && chunks <= 2 * kMost)) TS_WIDE(2);
+  else if (chunks <= 3 * kMost) TS_WIDE(3);
   else TS_WIDE(4);
 #undef TS_NARROW
 #undef TS_WIDE
