@@ -28,7 +28,8 @@ struct LinearArgs {
   void* out;
   int M, N, K;
   int64_t xs, ws, os;
-  int per;  // tile columns per part of K, where K is split over workgroups
+  int groups;  // workgroups of the launch (gridDim would be an implicit argument: 0.4 us of host time)
+  int per;     // tile columns per part of K, where K is split over workgroups
 };
 
 // 16 codes at any address (gfx950 takes unaligned vector loads).
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a
   // Workgroups go round-robin over the 8 XCDs: those of the same rows of W run on one of them, which
   // reads W once (22 x 3968 x 6656 11.0 us by a grid of two dimensions, 7.9 so; 54 x 1856 x 25664 in
   // one part 32.2 and 20.6).
-  const int xcd = blockIdx.x % 8, per = gridDim.x / 8, more = gridDim.x % 8;
+  const int xcd = blockIdx.x % 8, per = a.groups / 8, more = a.groups % 8;
   const int tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
   const int tn = tiles_m.quotient(tile), n0 = tn * BN, m0 = (tile - tn * tiles_m.by) * BM;
   int8_t* const slot = lds + kp * kUnit;
@@ -248,10 +249,11 @@ __global__ __launch_bounds__(8 * kWave) void int8_rows_kernel(const LinearArgs a
 }
 
 template <typename T, int NTW, int MT>
-static int launch_rows8(const LinearArgs& a, bool aligned, hipStream_t st) {
+static int launch_rows8(LinearArgs a, bool aligned, hipStream_t st) {
   const int64_t tn = (a.N + 16 * NTW - 1) / (16 * NTW), tm = (a.M + 16 * MT - 1) / (16 * MT);
   if (tm * tn > 1 << 22) return TS_EUNSUPPORTED;  // 2^31 threads
-  const dim3 grid(static_cast<unsigned>(tm * tn)), block(8 * kWave);
+  a.groups = static_cast<int>(tm * tn);
+  const dim3 grid(a.groups), block(8 * kWave);
   if (aligned) hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, true>), grid, block, 0, st, a, Divisor(static_cast<int>(tm)));
   else hipLaunchKernelGGL((int8_rows_kernel<T, NTW, MT, false>), grid, block, 0, st, a, Divisor(static_cast<int>(tm)));
   return launch_status();
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(GM * GN * kWave, 2) void int8_tile_kernel(LinearArg
   // bands of 4 tiles of x, so that the tiles running on it share rows of x and W in its L2.
   int tm, tn;
   {
-    const int total = gridDim.x, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
+    const int xcd = blockIdx.x % 8, per = a.groups / 8, more = a.groups % 8;
     int t = xcd * per + min(xcd, more) + blockIdx.x / 8;
     if constexpr (kPart) {
       const int part = t / (tiles_m * tiles_n), k0 = part * a.per * kCols;
@@ -501,11 +503,12 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const LinearArgs a, con
 }
 
 template <typename T, int MW, int NW, int GM, int GN, int kCols, int kStages>
-static int launch_tiles(const LinearArgs& a, hipStream_t st) {
+static int launch_tiles(LinearArgs a, hipStream_t st) {
   constexpr int BM = 32 * MW * GM, BN = 32 * NW * GN;
   const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
   if (tm * tn > 1 << 22) return TS_EUNSUPPORTED;  // 2^31 threads
-  hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kCols, kStages>), dim3(static_cast<unsigned>(tm * tn)),
+  a.groups = static_cast<int>(tm * tn);
+  hipLaunchKernelGGL((int8_tile_kernel<T, MW, NW, GM, GN, kCols, kStages>), dim3(a.groups),
                      dim3(GM * GN * kWave), 0, st, a, static_cast<int>(tm), static_cast<int>(tn));
   return launch_status();
 }
@@ -517,8 +520,9 @@ static int launch_parts(LinearArgs a, int parts, int32_t* sums, hipStream_t st) 
   LinearArgs part = a;
   part.out = sums;
   part.os = quads * 4;
+  part.groups = tm * tn * parts;
   part.per = ((a.K + kCols - 1) / kCols + parts - 1) / parts;
-  hipLaunchKernelGGL((int8_tile_kernel<int32_t, MW, NW, GM, GN, kCols, kStages>), dim3(tm * tn * parts),
+  hipLaunchKernelGGL((int8_tile_kernel<int32_t, MW, NW, GM, GN, kCols, kStages>), dim3(part.groups),
                      dim3(GM * GN * kWave), 0, st, part, tm, tn);
   if (const int rc = launch_status()) return rc;
   hipLaunchKernelGGL(int8_parts_kernel<T>, dim3((a.M * quads + 255) / 256), dim3(256), 0, st, a, sums, parts, quads);
@@ -572,17 +576,23 @@ struct Pick {
 // 297 x 4288 x 15680 68 and 47 (the same), 1257 x 3392 x 27328 247 and 144 (256 x 256, three), 137 x
 // 6464 x 18112 74 and 50 (256 x 256, eight); but 256 x 4096 x 4096 12.3 and 16.4, 1024 x 8192 x 8192
 // 83.7 and 85.1. Parts of the other shapes would add 0.2% over all the products.
+constexpr int kUnsplit = 4096;
 static Pick pick_kernel(int M, int N, int K, bool may_split) {
-  const int cus = compute_units();
-  const float k = static_cast<float>(K) / 1024.f, deep = k > 4.f ? k - 4.f : 0.f;
-  auto groups = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  auto times = [&](int64_t g) { return static_cast<float>((g + cus - 1) / cus); };  // workgroups per compute unit, one after another
-  constexpr int64_t kMost = 1 << 22;  // workgroups of 512 threads: a launch has fewer than 2^32
+  const unsigned cus = compute_units(), m = M, n = N;
+  const float k = static_cast<float>(K) / 1024.f, deep = K > kUnsplit ? k - 4.f : 0.f;
+  // 32-bit arithmetic, and constants in unrolled loops: this runs on the host at every call.
+  constexpr unsigned kMost = 1 << 22;  // workgroups of 512 threads: a launch has fewer than 2^32
+  auto groups = [&](unsigned bm, unsigned bn) {  // kMost + 1: more than that
+    const uint64_t g = static_cast<uint64_t>((m + bm - 1) / bm) * ((n + bn - 1) / bn);
+    return g > kMost ? kMost + 1 : static_cast<unsigned>(g);
+  };
+  auto times = [&](unsigned g) { return static_cast<float>((g + cus - 1) / cus); };  // workgroups per compute unit, one after another
   Pick best{0, 1};
   float least = 0.f;
+#pragma unroll
   for (int i = 0; i < 5; ++i) {
     const TileShape& t = kShapes[i];
-    const int64_t g = groups(t.bm, t.bn);
+    const unsigned g = groups(t.bm, t.bn);
     if (i > 0 && g > kMost) continue;
     const float us = times(g) * (t.fixed + t.per_k * k);
     if (i == 0 || us < least) {
@@ -591,26 +601,27 @@ static Pick pick_kernel(int M, int N, int K, bool may_split) {
     }
   }
   const TileShape& t = kShapes[best.kernel];
-  const int64_t g = groups(t.bm, t.bn);
+  const unsigned g = groups(t.bm, t.bn);
   least += 3.0f + times(g) * t.per_k * 1.2f * deep;
   if (g < cus) least += 0.5f * t.per_k * k;
+#pragma unroll
   for (int i = 0; i < 6; ++i) {
-    const int bm = 16 * kRowShapes[i].mt, bn = 16 * kRowShapes[i].ntw;
-    if (groups(bm, bn) > kMost) continue;
-    const float us = 3.f + times(groups(bm, bn)) * (kRowShapes[i].fixed + 0.018f * static_cast<float>(bm + bn) * (k + 0.3f * deep));
+    const unsigned bm = 16 * kRowShapes[i].mt, bn = 16 * kRowShapes[i].ntw, g = groups(bm, bn);
+    if (g > kMost) continue;
+    const float us = 3.f + times(g) * (kRowShapes[i].fixed + 0.018f * static_cast<float>(bm + bn) * (k + 0.3f * deep));
     if (us < least) {
       best.kernel = -1 - i;
       least = us;
     }
   }
-  if (!may_split || deep == 0.f) return best;
+  if (!may_split || K <= kUnsplit || least < 8.5f + kShapes[2].fixed) return best;
   const int columns = (K + 127) / 128;
   const float outputs = static_cast<float>(M) * static_cast<float>(N);
   for (int i : {0, 2}) {
     const TileShape& t = kShapes[i];
     for (int parts : {2, 3, 4, 6, 8}) {
       const int per = (columns + parts - 1) / parts;
-      const int64_t g = groups(t.bm, t.bn) * parts;
+      const unsigned g = groups(t.bm, t.bn) * parts;
       if ((parts - 1) * per >= columns || g > 4 * cus) continue;  // a part would be empty; nothing to fill
       if (g < cus / 4) continue;  // 16 x 16 x 131056 in 8 parts 57, as one workgroup of the row kernel 50
       const float us = 8.5f + times(g) * (t.fixed + 1.2f * t.per_k * static_cast<float>(per) / 8.f) +
@@ -668,7 +679,7 @@ static int launch_linear(const LinearArgs& a, bool padded, int32_t* sums, int64_
 using namespace ts;
 
 extern "C" int64_t ts_int8_linear_workspace(int M, int N, int K) {
-  if (M <= 0 || M > TS_INT8_MAX_DIM || N <= 0 || N > TS_INT8_MAX_DIM || K < 0 || K > TS_INT8_MAX_K) return 0;
+  if (M <= 0 || M > TS_INT8_MAX_DIM || N <= 0 || N > TS_INT8_MAX_DIM || K <= kUnsplit || K > TS_INT8_MAX_K) return 0;
   return parts_bytes(M, N, pick_kernel(M, N, K, true).parts);
 }
 
@@ -681,7 +692,7 @@ extern "C" int ts_int8_linear(const int8_t* x, int64_t x_stride, const float* x_
   if (dtype < TS_F32 || dtype > TS_BF16) return TS_EUNSUPPORTED;
   if (M == 0 || N == 0) return 0;
   if (!out || !x_scale || !w_scale || (K > 0 && (!x || !w))) return TS_EINVAL;
-  const LinearArgs a{x, w, x_scale, w_scale, out, M, N, K, x_stride, w_stride, o_stride, 0};
+  const LinearArgs a{x, w, x_scale, w_scale, out, M, N, K, x_stride, w_stride, o_stride, 0, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto* sums = static_cast<int32_t*>(workspace);
   switch (dtype) {

@@ -135,6 +135,7 @@ struct QuantArgs {
   int rows, N;
   int64_t xs, ys, qs;
   float eps;
+  int threads;  // of a workgroup (blockDim would be an implicit argument, which costs host time)
 };
 
 // CPT chunks of E elements per thread. LPR lanes of a wave on one row, a workgroup of 256 threads on
@@ -142,7 +143,7 @@ struct QuantArgs {
 template <typename T, int FORM, int LPR, int CPT>
 __global__ __launch_bounds__(LPR ? 256 : 1024) void quantize_rows_kernel(const QuantArgs a) {
   constexpr int E = Pack16<T>::N;
-  const int wave = threadIdx.x / kWave, TPR = LPR ? LPR : blockDim.x;
+  const int wave = threadIdx.x / kWave, TPR = LPR ? LPR : a.threads;
   const int64_t row = LPR ? static_cast<int64_t>(blockIdx.x) * (256 / (LPR ? LPR : 1)) + threadIdx.x / (LPR ? LPR : 1) : blockIdx.x;
   const int t = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
   if (LPR && row >= a.rows) return;
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(LPR ? 256 : 1024) void quantize_rows_kernel(const Q
 template <typename T, int FORM>
 __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs a) {
   const int64_t row = blockIdx.x;
-  const int N = a.N, wave = threadIdx.x / kWave, threads = blockDim.x;
+  const int N = a.N, wave = threadIdx.x / kWave, threads = a.threads;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   T* xo = static_cast<T*>(a.xo) + row * a.xs;
   const T* y = static_cast<const T*>(a.y) + row * a.ys;
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(1024) void quantize_rows_any_kernel(const QuantArgs
 }
 
 template <typename T, int FORM>
-static int launch_quantize(const QuantArgs& a, hipStream_t st) {
+static int launch_quantize(QuantArgs a, hipStream_t st) {
   constexpr int E = Pack16<T>::N;
   const int chunks = (a.N + E - 1) / E;
   // Wide rows: a workgroup of as many threads as there are chunks, up to 1024, then two to four
@@ -301,15 +302,18 @@ static int launch_quantize(const QuantArgs& a, hipStream_t st) {
   // 8.1; 32768 x 64 in 16 lanes each 4.0 and 6.9, in a wave each 10.5 and 15.1.
 #define TS_NARROW(L)                                                                                                 \
   hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, L, 1>), dim3((a.rows + 256 / (L) - 1) / (256 / (L))), dim3(256), 0, st, a)
-#define TS_WIDE(C)                                                                       \
-  hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, 0, C>), dim3(a.rows),                \
-                     dim3(((chunks + (C) - 1) / (C) + kWave - 1) / kWave * kWave), 0, st, a)
+#define TS_WIDE(C)                                                                                           \
+  do {                                                                                                       \
+    a.threads = ((chunks + (C) - 1) / (C) + kWave - 1) / kWave * kWave;                                      \
+    hipLaunchKernelGGL((quantize_rows_kernel<T, FORM, 0, C>), dim3(a.rows), dim3(a.threads), 0, st, a);      \
+  } while (0)
   constexpr int kMost = 1024;  // threads of a workgroup
   const int64_t much = FORM == kPlain ? 1 << 18 : FORM == kNorm ? 1 << 20 : INT64_MAX;  // chunks in all
   const bool two = chunks > kMost || (chunks >= 256 && static_cast<int64_t>(a.rows) * chunks >= much);
-  if (a.N < E || chunks > 4 * kMost)
-    hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(a.N < E ? kWave : kMost), 0, st, a);
-  else if (chunks <= 16) TS_NARROW(16);
+  if (a.N < E || chunks > 4 * kMost) {
+    a.threads = a.N < E ? kWave : kMost;
+    hipLaunchKernelGGL((quantize_rows_any_kernel<T, FORM>), dim3(a.rows), dim3(a.threads), 0, st, a);
+  } else if (chunks <= 16) TS_NARROW(16);
   else if (chunks <= 32) TS_NARROW(32);
   else if (chunks <= 64) TS_NARROW(64);
   else if (!two) TS_WIDE(1);
@@ -343,6 +347,8 @@ static int launch_form(QuantArgs a, int form, hipStream_t st) {
 // ---- rows of an 8-bit table -----------------------------------------------------------------
 // out[t] = (T)(q[ids[t]] * scale[ids[t]]): one thread per 16 codes. Bound by HBM (and, for few
 // ids, by the chain id -> row). An id outside the table gives a row of NaN.
+constexpr int kMostBlocks = 1 << 20;  // of a launch; one of fewer has a thread for every 16 bytes
+
 struct TableArgs {
   const int8_t* q;
   const float* scale;
@@ -356,7 +362,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void int8_embedding_kernel(const TableArgs a) {
   const int N = a.N;
   const int64_t total = static_cast<int64_t>(a.rows) * a.per_row;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += kMostBlocks * 256ll) {
     const int64_t t = u / a.per_row;
     const int i = static_cast<int>(u - t * a.per_row) * 16;
     const int64_t id = a.ids ? a.ids[t] : t;
@@ -395,7 +401,7 @@ struct PadArgs {
 
 __global__ __launch_bounds__(256) void int8_pad_rows_kernel(const PadArgs p) {
   const int64_t total = (static_cast<int64_t>(p.a_rows) + p.b_rows) * p.per_row;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < total; u += kMostBlocks * 256ll) {
     const int64_t row = u / p.per_row;
     const int i = static_cast<int>(u - row * p.per_row) * 16;
     const bool first = row < p.a_rows;
@@ -421,7 +427,7 @@ template <typename T>
 static int launch_embedding(TableArgs a, hipStream_t st) {
   a.per_row = (a.N + 15) / 16;
   const int64_t blocks = (static_cast<int64_t>(a.rows) * a.per_row + 255) / 256;
-  hipLaunchKernelGGL(int8_embedding_kernel<T>, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256),
+  hipLaunchKernelGGL(int8_embedding_kernel<T>, dim3(static_cast<unsigned>(blocks < kMostBlocks ? blocks : kMostBlocks)), dim3(256),
                      0, st, a);
   return launch_status();
 }
@@ -452,7 +458,7 @@ extern "C" int ts_int8_quantize_rows(void* x, const void* y, const void* w, int8
       if (T == 1 || x_stride != y_stride || d < N * es || d > pitch - N * es) return TS_EINVAL;
     }
   }
-  const QuantArgs a{x, x, y, w, q, scale, T, N, x_stride, y_stride, q_stride, eps};
+  const QuantArgs a{x, x, y, w, q, scale, T, N, x_stride, y_stride, q_stride, eps, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case TS_F32: return launch_form<float>(a, form, st);
@@ -488,7 +494,7 @@ extern "C" int ts_int8_pad_rows(const int8_t* a, int64_t a_stride, int8_t* a_out
   if ((a_rows > 0 && (!a || !a_out)) || (b_rows > 0 && (!b || !b_out))) return TS_EINVAL;
   const PadArgs p{a, b, a_out, b_out, a_stride, b_stride, o_stride, a_rows, b_rows, N, static_cast<int>(padded / 16)};
   const int64_t blocks = ((static_cast<int64_t>(a_rows) + b_rows) * p.per_row + 255) / 256;
-  hipLaunchKernelGGL(int8_pad_rows_kernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0,
+  hipLaunchKernelGGL(int8_pad_rows_kernel, dim3(static_cast<unsigned>(blocks < kMostBlocks ? blocks : kMostBlocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), p);
   return launch_status();
 }
